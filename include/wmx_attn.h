@@ -39,7 +39,7 @@
 extern "C" {
 #endif
 
-#define WMX_ABI_VERSION 15
+#define WMX_ABI_VERSION 16
 
 enum {
   WMX_OK = 0,
@@ -713,6 +713,177 @@ typedef struct wmx_plan_args {
   int32_t num_f_units;
 } wmx_plan_args;
 
+/*
+ * Quantised KV pool. A pool row (one slot of one head, D values) is D codes and
+ * one fp32 scale: value = code * scale with codes in e4m3 (OCP, magnitudes up
+ * to 448) or int8 (up to 127). A row x is stored with scale = max|x| / T and
+ * code = x * (T / max|x|) rounded to nearest even (T the largest code); a row
+ * whose largest magnitude is below 2^-100 as zeros with scale 0, a row that
+ * holds an infinity or a NaN as zero codes with scale NaN, so that it reads
+ * back as NaN.
+ */
+enum {
+  WMX_POOL_BF16 = 0, /* no codes: bf16 values (wmx_tree_attn only) */
+  WMX_POOL_E4M3 = 1,
+  WMX_POOL_INT8 = 2
+};
+
+/*
+ * Quantising pool write: rows of keys, rope(rms_norm(key) * weight), and of
+ * values, both computed in fp32 without intermediate rounding, quantised into
+ * pool slots. Either side may be absent (key and key_codes NULL, or value and
+ * value_codes). Token t of batch row b goes to slot slots[b * slots_stride + t]
+ * (slots NULL: slot t); a slot outside [0, pool_slots) is skipped. Without
+ * weight, cos and sin (all NULL) the keys are quantised as they are.
+ * Element strides [batch, channel, head, token or slot]; code strides in bytes,
+ * multiples of 8, unit stride along D; sources 16-byte aligned rows as
+ * wmx_kv_store_args. head_dim 64, 96 or 128.
+ */
+typedef struct wmx_kv_quant_args {
+  const void* key;
+  const void* value;
+  const void* k_norm_weight; /* (C, D) */
+  const void* cos;           /* (B, T, D), or (N, D) read at the slot with rope_by_slot */
+  const void* sin;
+  const int64_t* slots;
+  void* key_codes;
+  void* value_codes;
+  float* key_scales;
+  float* value_scales;
+  int64_t key_stride[4];
+  int64_t value_stride[4];
+  int64_t key_codes_stride[4];
+  int64_t value_codes_stride[4];
+  int64_t key_scales_stride[4];
+  int64_t value_scales_stride[4];
+  int64_t rope_stride[2];
+  int64_t slots_stride;
+  int32_t key_dtype;         /* WMX_DTYPE_F32 or WMX_DTYPE_BF16 */
+  int32_t value_dtype;
+  int32_t weight_dtype;
+  int32_t rope_dtype;
+  int32_t format;            /* WMX_POOL_E4M3 or WMX_POOL_INT8 */
+  int32_t batch;
+  int32_t channels;
+  int32_t heads;
+  int32_t tokens;
+  int32_t head_dim;
+  int32_t pool_slots;
+  int32_t rope_by_slot;
+  float eps;
+} wmx_kv_quant_args;
+
+/*
+ * Pool rows read back: out[b, c, h, t] = bf16(codes * scale) of slot
+ * slots[b * slots_stride + t] (slots NULL: slot t), zeros for a slot outside
+ * [0, pool_slots). out is (B, C, H, T, D) contiguous, 16-byte aligned.
+ */
+typedef struct wmx_kv_read_args {
+  const void* codes;
+  const float* scales;
+  const int64_t* slots;
+  void* out;
+  int64_t codes_stride[4];
+  int64_t scales_stride[4];
+  int64_t slots_stride;
+  int32_t format;
+  int32_t batch;
+  int32_t channels;
+  int32_t heads;
+  int32_t tokens;
+  int32_t head_dim;
+  int32_t pool_slots;
+} wmx_kv_read_args;
+
+/*
+ * Attention of `nodes` query tokens per batch row (a tree of drafted tokens, or
+ * one token) over a KV pool. Row b has base_b = use_dummy + kv_lengths[b]
+ * committed slots (kv_length_scalar without kv_lengths; negative lengths count
+ * as 0); its drafted tokens sit behind them, node a at slot base_b + a. Query
+ * node i sees slot j < base_b, and slot base_b + a where tree_mask[b, i, a]
+ * (no node without tree_mask), and of these the ones with key_mask[b, j] when
+ * key_mask is given. Slots at or past `capacity` are never read. Rows with no
+ * visible slot produce zeros.
+ * q (B, Hq, n, D) and o in bf16, strides [batch, head, node]; k/v pool strides
+ * [batch, head, slot] in elements of the format, scales [batch, head] with unit
+ * stride along the slots (WMX_POOL_BF16: none). Rows of q and of a bf16 pool
+ * are 16-byte aligned, rows of codes 8-byte aligned (16 for head_dim 64 and
+ * 128), o 4-byte; a slot stride is below 2^25 bytes.
+ */
+typedef struct wmx_tree_args {
+  const void* q;
+  const void* k;
+  const void* v;
+  const float* k_scales;
+  const float* v_scales;
+  void* o;
+  const int64_t* kv_lengths;
+  const uint8_t* tree_mask;  /* bytes, strides [batch, node], unit along the ancestors */
+  const uint8_t* key_mask;   /* bytes (B, N), unit stride along the slots */
+  void* workspace;           /* wmx_tree_workspace_size bytes, 16-byte aligned */
+  int64_t workspace_bytes;
+  int64_t kv_length_scalar;
+  int64_t q_stride[3];
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  int64_t o_stride[3];
+  int64_t k_scales_stride[2];
+  int64_t v_scales_stride[2];
+  int64_t tree_mask_stride[2];
+  int64_t key_mask_stride;
+  int32_t format;            /* WMX_POOL_* */
+  int32_t batch;
+  int32_t q_heads;
+  int32_t kv_heads;
+  int32_t nodes;
+  int32_t capacity;          /* pool slots N */
+  int32_t head_dim;          /* 64, 96 or 128 */
+  int32_t use_dummy;
+  int32_t num_splits;        /* key splits; 0 chooses */
+  float softmax_scale;       /* positive */
+} wmx_tree_args;
+
+/*
+ * Log probabilities of given tokens, entropy and top alternatives of rows of
+ * logits, and their gradient.
+ *   lse = log sum_j exp(x_j), log_probs = x[token] - lse,
+ *   entropy = lse - sum_j p_j x_j, top: the top_k largest x (equal values: the
+ *   lower index first; NaN above all) as x - lse with their indices.
+ * A token equal to ignore_index gives log_probs 0 and no gradient, another
+ * token outside [0, vocab) NaN. A row of -inf only gives -inf log
+ * probabilities, entropy 0 and no gradient; a row with a NaN or +inf gives NaN.
+ * Gradient: with s the sum of the row's log probability gradients,
+ *   dx_j = -p_j (s + grad_entropy (x_j - lse + entropy))
+ *          + grad_log_probs [j == token] + sum_i grad_top[i] [j == top_indices[i]];
+ * absent gradients (NULL) are zero. Rows are row_stride elements apart with
+ * unit stride along the vocabulary, any alignment of the element type;
+ * grad_logits is (rows, vocab) contiguous, of the logits' type.
+ */
+enum { WMX_DTYPE_F16 = 2 }; /* logits only */
+#define WMX_SCORE_MAX_TOP_K 32
+
+typedef struct wmx_score_args {
+  const void* logits;
+  const int64_t* tokens;     /* (rows) */
+  float* log_probs;          /* (rows); gradient: unused */
+  float* entropy;            /* (rows); gradient: read */
+  float* lse;                /* (rows); gradient: read */
+  float* top_log_probs;      /* (rows, top_k); gradient: unused */
+  int64_t* top_indices;      /* (rows, top_k); gradient: read */
+  const float* grad_log_probs;
+  const float* grad_entropy;
+  const float* grad_top;     /* (rows, top_k) */
+  void* grad_logits;
+  void* workspace;           /* wmx_score_workspace_size bytes, 16-byte aligned */
+  int64_t workspace_bytes;
+  int64_t rows;
+  int64_t row_stride;
+  int64_t ignore_index;
+  int32_t vocab;             /* 1 .. 2^31 - 2^16 */
+  int32_t top_k;             /* 0 .. min(vocab, WMX_SCORE_MAX_TOP_K) */
+  int32_t dtype;             /* WMX_DTYPE_F32, WMX_DTYPE_BF16 or WMX_DTYPE_F16 */
+} wmx_score_args;
+
 /* Library identity and struct layout checks for FFI bindings. */
 int wmx_abi_version(void);
 size_t wmx_attn_args_size(void);
@@ -857,6 +1028,21 @@ int64_t wmx_plan_workspace_size(const wmx_plan_args* args);
 int64_t wmx_plan_unit_workspace_size(const wmx_plan_args* args);
 int wmx_plan_count(const wmx_plan_args* args, void* stream);
 int wmx_plan_fill(const wmx_plan_args* args, void* stream);
+
+/* Quantised KV pool (see wmx_kv_quant_args, wmx_kv_read_args) and the attention
+ * of drafted tokens over a pool (see wmx_tree_args): no counterpart in the
+ * reference, whose pools are bf16 and whose decode takes one token. */
+int wmx_kv_quant_store(const wmx_kv_quant_args* args, void* stream);
+int wmx_kv_quant_read(const wmx_kv_read_args* args, void* stream);
+int32_t wmx_tree_num_splits(const wmx_tree_args* args);
+int64_t wmx_tree_workspace_size(const wmx_tree_args* args);
+int wmx_tree_attn(const wmx_tree_args* args, void* stream);
+
+/* Scores of given tokens and their gradient (see wmx_score_args); outputs are
+ * fully overwritten. */
+int64_t wmx_score_workspace_size(const wmx_score_args* args);
+int wmx_score(const wmx_score_args* args, void* stream);
+int wmx_score_bwd(const wmx_score_args* args, void* stream);
 
 #ifdef __cplusplus
 }

@@ -68,16 +68,29 @@ def _torch_flags() -> tuple[list[str], list[str]]:
 
 
 def build_ops(verbose: bool = False) -> Path:
-    """Compile the C++ operator registrations (csrc/torch_ops.cpp, host code
-    only) against libtorch and libwmx_attn.so into libwmx_torch.so."""
+    """Compile the C++ operator registrations (csrc/*.cpp, host code only)
+    against libtorch and libwmx_attn.so into libwmx_torch.so."""
     compile_flags, link_flags = _torch_flags()
+    compiler = os.environ.get("CXX", "g++")
+    obj_dir = OPS_LIBRARY.parent / "obj"
+    obj_dir.mkdir(parents=True, exist_ok=True)
+
+    def run(cmd: list[str]) -> None:
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        proc = subprocess.run(cmd, capture_output=True, text=True)
+        if proc.returncode != 0:
+            raise RuntimeError(f"building libwmx_torch.so failed:\n{proc.stderr}")
+
+    def compile_one(src: Path) -> Path:
+        obj = obj_dir / (src.stem + ".cpp.o")
+        run([compiler, *compile_flags, "-c", str(src), "-o", str(obj)])
+        return obj
+
+    with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:
+        objects = list(pool.map(compile_one, sorted(CSRC.glob("*.cpp"))))
     tmp = OPS_LIBRARY.with_suffix(".so.tmp")
-    cmd = [os.environ.get("CXX", "g++"), *compile_flags, "-shared", str(CSRC / "torch_ops.cpp"), "-o", str(tmp), *link_flags]
-    if verbose:
-        print(" ".join(cmd), flush=True)
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        raise RuntimeError(f"building libwmx_torch.so failed:\n{proc.stderr}")
+    run([compiler, "-shared", *map(str, objects), "-o", str(tmp), *link_flags])
     os.replace(tmp, OPS_LIBRARY)
     return OPS_LIBRARY
 

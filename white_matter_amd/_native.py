@@ -19,7 +19,7 @@ import torch
 LIBRARY = Path(__file__).resolve().parent / "lib" / "libwmx_attn.so"
 # the operators registered from C++ (csrc/torch_ops.cpp), linked against LIBRARY
 OPS_LIBRARY = Path(__file__).resolve().parent / "lib" / "libwmx_torch.so"
-ABI_VERSION = 15
+ABI_VERSION = 16
 
 _c_i64_3 = ctypes.c_int64 * 3
 _c_i64_2 = ctypes.c_int64 * 2
@@ -336,6 +336,9 @@ class KvMixBwdArgs(ctypes.Structure):
     ]
 
 
+# most top alternatives of a score (WMX_SCORE_MAX_TOP_K)
+SCORE_MAX_TOP_K = 32
+
 # wmx_plan_args counts (WMX_PLAN_*): the columns that the host reads by name
 PLAN_COUNTS = 17
 PLAN_REFUSED, PLAN_GENERAL = 1, 2
@@ -433,6 +436,14 @@ EXPORTS = (
     "wmx_plan_unit_workspace_size",
     "wmx_plan_count",
     "wmx_plan_fill",
+    "wmx_kv_quant_store",
+    "wmx_kv_quant_read",
+    "wmx_tree_num_splits",
+    "wmx_tree_workspace_size",
+    "wmx_tree_attn",
+    "wmx_score_workspace_size",
+    "wmx_score",
+    "wmx_score_bwd",
 )
 
 

@@ -2,6 +2,7 @@
 // Each entry point checks what the kernels assume about shapes, strides and
 // alignment before anything is launched, so a bad call returns an error code
 // instead of reaching the GPU.
+#include <climits>
 #include <cstdarg>
 #include <cstdio>
 #include <cstring>
@@ -668,6 +669,132 @@ int wmx_decode_noalloc(const wmx_decode_args* a, void* stream) {
   b.workspace_bytes = kDecodeScratchBytes;
   b.counters = nullptr;  // the splits are merged by a second kernel
   return launched(wmx::launch_decode(b, (hipStream_t)stream));
+}
+
+static bool pool_codes(int32_t format) { return format == WMX_POOL_E4M3 || format == WMX_POOL_INT8; }
+
+int wmx_kv_quant_store(const wmx_kv_quant_args* a, void* stream) {
+  if (!a) return fail(WMX_E_INVALID, "args is NULL");
+  if (a->head_dim != 64 && a->head_dim != 96 && a->head_dim != 128)
+    return fail(WMX_E_UNSUPPORTED, "pool head_dim %d is not 64, 96 or 128", a->head_dim);
+  if (!pool_codes(a->format)) return fail(WMX_E_INVALID, "format must be WMX_POOL_E4M3 or WMX_POOL_INT8");
+  if (a->batch < 0 || a->channels < 0 || a->heads < 0 || a->tokens < 0 || a->pool_slots < 0)
+    return fail(WMX_E_INVALID, "negative shape");
+  for (int dt : {a->key_dtype, a->value_dtype, a->weight_dtype, a->rope_dtype})
+    if (dt != WMX_DTYPE_F32 && dt != WMX_DTYPE_BF16) return fail(WMX_E_INVALID, "dtype must be WMX_DTYPE_F32 or WMX_DTYPE_BF16");
+  if (!(a->eps >= 0.f)) return fail(WMX_E_INVALID, "eps must be >= 0");
+  if ((int64_t)a->batch * a->channels * a->tokens * a->heads == 0) return WMX_OK;
+  if (!a->key && !a->value) return fail(WMX_E_INVALID, "quantised store has neither keys nor values");
+  if (!a->key != !a->key_codes || !a->key != !a->key_scales || !a->value != !a->value_codes || !a->value != !a->value_scales)
+    return fail(WMX_E_INVALID, "a side's rows, codes and scales are given together");
+  if (!a->k_norm_weight != !a->cos || !a->cos != !a->sin || (a->cos && !a->key))
+    return fail(WMX_E_INVALID, "the norm weight, cos and sin are given together, with keys");
+  if (!a->slots && a->tokens > a->pool_slots) return fail(WMX_E_INVALID, "more tokens than slots, and no slots given");
+  if (!aligned16(a->key) || !aligned16(a->value) || !aligned16(a->k_norm_weight) || !aligned16(a->cos) || !aligned16(a->sin) ||
+      !aligned8(a->slots) || !aligned8(a->key_codes) || !aligned8(a->value_codes))
+    return fail(WMX_E_INVALID, "quantised store operands must be 16-byte aligned, codes 8-byte");
+  if (!strides_vec8(a->key_stride, 4) || !strides_vec8(a->value_stride, 4) || !strides_vec8(a->key_codes_stride, 4) ||
+      !strides_vec8(a->value_codes_stride, 4) || !strides_vec8(a->rope_stride, 2))
+    return fail(WMX_E_INVALID, "quantised store strides must be multiples of 8 elements");
+  return launched(wmx::launch_kv_quant(*a, (hipStream_t)stream));
+}
+
+int wmx_kv_quant_read(const wmx_kv_read_args* a, void* stream) {
+  if (!a) return fail(WMX_E_INVALID, "args is NULL");
+  if (a->head_dim != 64 && a->head_dim != 96 && a->head_dim != 128)
+    return fail(WMX_E_UNSUPPORTED, "pool head_dim %d is not 64, 96 or 128", a->head_dim);
+  if (!pool_codes(a->format)) return fail(WMX_E_INVALID, "format must be WMX_POOL_E4M3 or WMX_POOL_INT8");
+  if (a->batch < 0 || a->channels < 0 || a->heads < 0 || a->tokens < 0 || a->pool_slots < 0)
+    return fail(WMX_E_INVALID, "negative shape");
+  if ((int64_t)a->batch * a->channels * a->tokens * a->heads == 0) return WMX_OK;
+  if (!a->codes || !a->scales || !a->out) return fail(WMX_E_INVALID, "pool read pointer is NULL");
+  if (!aligned16(a->out) || !aligned8(a->codes) || !aligned8(a->slots) || !strides_vec8(a->codes_stride, 4))
+    return fail(WMX_E_INVALID, "pool codes must be 8-byte aligned rows, the output 16-byte aligned");
+  return launched(wmx::launch_kv_read(*a, (hipStream_t)stream));
+}
+
+static int check_tree(const wmx_tree_args* a) {
+  if (!a) return fail(WMX_E_INVALID, "args is NULL");
+  if (a->head_dim != 64 && a->head_dim != 96 && a->head_dim != 128)
+    return fail(WMX_E_UNSUPPORTED, "head_dim %d is not 64, 96 or 128", a->head_dim);
+  if (a->format != WMX_POOL_BF16 && !pool_codes(a->format)) return fail(WMX_E_INVALID, "pool format %d", a->format);
+  if (a->batch < 0 || a->q_heads <= 0 || a->kv_heads <= 0 || a->nodes < 0 || a->capacity < 0 || a->num_splits < 0)
+    return fail(WMX_E_INVALID, "negative or zero shape");
+  if (a->q_heads % a->kv_heads != 0) return fail(WMX_E_INVALID, "q_heads %% kv_heads != 0");
+  if ((int64_t)a->nodes * (a->q_heads / a->kv_heads) > (1 << 24))
+    return fail(WMX_E_UNSUPPORTED, "more than 2^24 query rows per KV head");
+  if (a->capacity > INT32_MAX - (1 << 20)) return fail(WMX_E_UNSUPPORTED, "pool of %d slots", a->capacity);
+  if (a->use_dummy != 0 && a->use_dummy != 1) return fail(WMX_E_INVALID, "use_dummy must be 0 or 1");
+  if (!(a->softmax_scale > 0.f) || a->softmax_scale > 3.0e38f)
+    return fail(WMX_E_UNSUPPORTED, "softmax_scale must be positive and finite");
+  return WMX_OK;
+}
+
+int32_t wmx_tree_num_splits(const wmx_tree_args* a) { return check_tree(a) ? 0 : wmx::tree_num_splits(*a); }
+int64_t wmx_tree_workspace_size(const wmx_tree_args* a) { return check_tree(a) ? 0 : wmx::tree_workspace_size(*a); }
+
+int wmx_tree_attn(const wmx_tree_args* a, void* stream) {
+  if (const int rc = check_tree(a)) return rc;
+  if (a->batch == 0 || a->nodes == 0) return WMX_OK;
+  const bool codes = a->format != WMX_POOL_BF16;
+  if (!a->q || !a->o || (a->capacity > 0 && (!a->k || !a->v || (codes && (!a->k_scales || !a->v_scales)))))
+    return fail(WMX_E_INVALID, "tree attention pointer is NULL");
+  if (!aligned16(a->q) || !strides_vec8(a->q_stride, 3)) return fail(WMX_E_INVALID, "q must be 16-byte aligned rows");
+  if (((uintptr_t)a->o & 3u) || a->o_stride[0] % 2 || a->o_stride[1] % 2 || a->o_stride[2] % 2)
+    return fail(WMX_E_INVALID, "o must be 4-byte aligned rows");
+  // rows of codes are read 16 bytes at a time, at head_dim 96 8 bytes
+  const int64_t unit = !codes ? 8 : a->head_dim == 96 ? 8 : 16;
+  const uintptr_t low = (codes && a->head_dim == 96) ? 7u : 15u;
+  if (((uintptr_t)a->k & low) || ((uintptr_t)a->v & low)) return fail(WMX_E_INVALID, "pool rows must be 16-byte aligned");
+  for (const int64_t* st : {a->k_stride, a->v_stride}) {
+    for (int i = 0; i < 3; ++i)
+      if (st[i] % unit) return fail(WMX_E_INVALID, "pool rows must be 16-byte aligned");
+    if (st[2] < 0 || st[2] * (codes ? 1 : 2) >= (1 << 25))
+      return fail(WMX_E_UNSUPPORTED, "pool slots must lie less than 2^25 bytes apart");
+  }
+  const int64_t need = wmx::tree_workspace_size(*a);
+  if (need > 0 && (!a->workspace || a->workspace_bytes < need || !aligned16(a->workspace)))
+    return fail(WMX_E_WORKSPACE, "tree attention needs %lld workspace bytes", (long long)need);
+  return launched(wmx::launch_tree(*a, (hipStream_t)stream));
+}
+
+static int check_score(const wmx_score_args* a) {
+  if (!a) return fail(WMX_E_INVALID, "args is NULL");
+  if (a->dtype != WMX_DTYPE_F32 && a->dtype != WMX_DTYPE_BF16 && a->dtype != WMX_DTYPE_F16)
+    return fail(WMX_E_INVALID, "logits must be fp32, bf16 or fp16");
+  if (a->rows < 0 || a->vocab < 1 || a->vocab > INT32_MAX - 65536) return fail(WMX_E_INVALID, "score shape");
+  if (a->top_k < 0 || a->top_k > WMX_SCORE_MAX_TOP_K || a->top_k > a->vocab)
+    return fail(WMX_E_UNSUPPORTED, "top_k %d is not in [0, %d]", a->top_k,
+                a->vocab < WMX_SCORE_MAX_TOP_K ? a->vocab : WMX_SCORE_MAX_TOP_K);
+  if (a->rows > 0) {
+    if (!a->logits || !a->tokens || !a->entropy || !a->lse || (a->top_k && !a->top_indices))
+      return fail(WMX_E_INVALID, "score pointer is NULL");
+    if (((uintptr_t)a->logits & (a->dtype == WMX_DTYPE_F32 ? 3u : 1u)) || !aligned8(a->tokens) || !aligned8(a->top_indices))
+      return fail(WMX_E_INVALID, "score operands must be aligned to their elements");
+  }
+  return WMX_OK;
+}
+
+int64_t wmx_score_workspace_size(const wmx_score_args* a) {
+  return a && a->rows > 0 && a->vocab > 0 && a->top_k >= 0 ? wmx::score_workspace_size(*a) : 0;
+}
+
+int wmx_score(const wmx_score_args* a, void* stream) {
+  if (const int rc = check_score(a)) return rc;
+  if (a->rows == 0) return WMX_OK;
+  if (!a->log_probs || (a->top_k && !a->top_log_probs)) return fail(WMX_E_INVALID, "score pointer is NULL");
+  const int64_t need = wmx::score_workspace_size(*a);
+  if (need > 0 && (!a->workspace || a->workspace_bytes < need || !aligned16(a->workspace)))
+    return fail(WMX_E_WORKSPACE, "scores need %lld workspace bytes", (long long)need);
+  return launched(wmx::launch_score(*a, (hipStream_t)stream));
+}
+
+int wmx_score_bwd(const wmx_score_args* a, void* stream) {
+  if (const int rc = check_score(a)) return rc;
+  if (a->rows == 0) return WMX_OK;
+  if (!a->grad_logits || ((uintptr_t)a->grad_logits & (a->dtype == WMX_DTYPE_F32 ? 3u : 1u)))
+    return fail(WMX_E_INVALID, "grad_logits must be aligned to its elements");
+  return launched(wmx::launch_score_bwd(*a, (hipStream_t)stream));
 }
 
 }  // extern "C"

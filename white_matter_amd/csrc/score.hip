@@ -1,0 +1,433 @@
+// Log probabilities of given tokens, entropy and top alternatives of rows of
+// logits, and their gradient (formulas in wmx_attn.h). HBM-bound: the forward
+// reads each logit once, the gradient reads it once more and writes it once.
+//
+// Forward: a workgroup takes one chunk of a row, 32 KB that its 256 threads
+// hold in registers (eight 16-byte loads each, all in flight at once), so the
+// maximum, the sums and the selection pass over registers and not over memory
+// again. A chunk leaves (max m, s = sum exp(x - m), t = sum exp(x - m)(x - m))
+// and its own top_k, which a second kernel merges per row: with M the largest
+// m and S = sum s_c exp(m_c - M), lse = M + log S and
+// entropy = log S - sum exp(m_c - M)(t_c + s_c (m_c - M)) / S.
+// Everything is fp32; p_j x_j is summed relative to the maximum, so entropies
+// of peaked rows do not cancel.
+#include "wmx_kernels.h"
+
+namespace wmx {
+
+typedef u32x4 u32x4_any __attribute__((aligned(2)));  // rows of odd vocabularies start anywhere
+
+constexpr int kScoreThreads = 256;
+constexpr int kScoreLoads = 8;                    // 16-byte loads per thread and chunk
+constexpr int kScoreCandidates = 512;             // room for a chunk's possible top entries
+constexpr float kFarBelow = -1.0e4f;              // exp of it is zero; keeps -inf * 0 out of the entropy
+
+template <int DT>
+struct Logit {
+  static constexpr int kPer = DT == WMX_DTYPE_F32 ? 4 : 8;  // elements of 16 bytes
+  static constexpr int kChunk = kScoreThreads * kScoreLoads * kPer;
+  static constexpr int kSize = DT == WMX_DTYPE_F32 ? 4 : 2;
+
+  static __device__ __forceinline__ float one(const void* row, int64_t j) {
+    if constexpr (DT == WMX_DTYPE_F32) return ((const float*)row)[j];
+    else if constexpr (DT == WMX_DTYPE_BF16) return (float)((const bf16*)row)[j];
+    else return (float)((const _Float16*)row)[j];
+  }
+  static __device__ __forceinline__ void unpack(const u32x4& w, float (&x)[kPer]) {
+    if constexpr (DT == WMX_DTYPE_F32) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = __uint_as_float(w[e]);
+    } else if constexpr (DT == WMX_DTYPE_BF16) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[2 * e] = bf16_lo(w[e]);
+        x[2 * e + 1] = bf16_hi(w[e]);
+      }
+    } else {
+      typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+      const f16x8 h = __builtin_bit_cast(f16x8, w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = (float)h[e];
+    }
+  }
+  static __device__ __forceinline__ u32x4 pack(const float (&x)[kPer]) {
+    if constexpr (DT == WMX_DTYPE_F32) {
+      return u32x4{__float_as_uint(x[0]), __float_as_uint(x[1]), __float_as_uint(x[2]), __float_as_uint(x[3])};
+    } else if constexpr (DT == WMX_DTYPE_BF16) {
+      return u32x4{pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7])};
+    } else {
+      typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+      f16x8 h;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) h[e] = (_Float16)x[e];
+      return __builtin_bit_cast(u32x4, h);
+    }
+  }
+  static __device__ __forceinline__ void put(void* row, int64_t j, float x) {
+    if constexpr (DT == WMX_DTYPE_F32) ((float*)row)[j] = x;
+    else if constexpr (DT == WMX_DTYPE_BF16) ((bf16*)row)[j] = (bf16)x;
+    else ((_Float16*)row)[j] = (_Float16)x;
+  }
+  // The vector at element j of a row, -inf past its end.
+  static __device__ __forceinline__ u32x4 load(const void* row, int64_t j, int64_t vocab) {
+    if (j + kPer <= vocab) {
+      return __builtin_nontemporal_load((const u32x4_any*)((const char*)row + j * kSize));
+    }
+    float x[kPer];
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) x[e] = j + e < vocab ? one(row, j + e) : kNegInf;
+    return pack(x);
+  }
+};
+
+// A float's place in the order of the top entries: larger is earlier, NaN
+// first, -0 and 0 alike.
+__device__ __forceinline__ uint32_t order_of(float x) {
+  const uint32_t u = __float_as_uint(x + 0.f);
+  if (x != x) return 0xffffffffu;
+  return (u >> 31) ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float value_of(uint32_t order) {
+  if (order == 0xffffffffu) return __builtin_nanf("");
+  return __uint_as_float((order >> 31) ? order & 0x7fffffffu : ~order);
+}
+// (value, index) as one key: a larger key is an earlier entry.
+__device__ __forceinline__ uint64_t entry_key(float x, int64_t j) {
+  return ((uint64_t)order_of(x) << 32) | (uint32_t)~(uint32_t)j;
+}
+__device__ __forceinline__ int64_t entry_index(uint64_t key) { return (int64_t)(uint32_t)~(uint32_t)key; }
+
+template <class T, class Op>
+__device__ __forceinline__ T wave_reduce(T x, Op op) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) x = op(x, __shfl_xor(x, o));
+  return x;
+}
+template <class T, class Op>
+__device__ __forceinline__ T block_reduce(T x, T* lds, Op op) {
+  x = wave_reduce(x, op);
+  const int w = threadIdx.x >> 6;
+  __syncthreads();  // earlier readers of lds are done
+  if ((threadIdx.x & 63) == 0) lds[w] = x;
+  __syncthreads();
+  T r = lds[0];
+#pragma unroll
+  for (int i = 1; i < kScoreThreads / 64; ++i) r = op(r, lds[i]);
+  return r;
+}
+
+struct ScorePart {
+  float m, s, t, pad;
+};
+
+// Writes a row's results from its merged statistics and sorted entries.
+__device__ __forceinline__ void finish_row(const wmx_score_args& a, int64_t row, float m, float s, float t, float x_token) {
+  const bool empty = m == kNegInf && s == 0.f;
+  const float log_s = logf(s);
+  const float lse = empty ? kNegInf : m + log_s;
+  a.lse[row] = lse;
+  a.entropy[row] = empty ? 0.f : log_s - t / s;
+  const int64_t token = a.tokens[row];
+  float lp;
+  if (token == a.ignore_index) lp = 0.f;
+  else if (token < 0 || token >= a.vocab) lp = __builtin_nanf("");
+  else lp = empty ? kNegInf : (x_token - m) - log_s;
+  a.log_probs[row] = lp;
+}
+
+template <int DT>
+__device__ __forceinline__ float token_logit(const wmx_score_args& a, const void* base, int64_t row) {
+  const int64_t token = a.tokens[row];
+  return token >= 0 && token < a.vocab ? Logit<DT>::one(base, token) : 0.f;
+}
+
+// One chunk of one row. TOP: whether entries are selected.
+template <int DT, bool TOP>
+__global__ __launch_bounds__(kScoreThreads) void score_kernel(const wmx_score_args a, int chunks) {
+  using L = Logit<DT>;
+  constexpr int P = L::kPer;
+  __shared__ float red[kScoreThreads / 64];
+  const int64_t row = blockIdx.x / chunks;
+  const int chunk = (int)(blockIdx.x - row * chunks);
+  const int tid = threadIdx.x;
+  const void* base = (const char*)a.logits + row * a.row_stride * L::kSize;
+  const int64_t j0 = (int64_t)chunk * L::kChunk + tid * P;  // this thread's vectors: j0 + i * 256 P
+
+  u32x4 w[kScoreLoads];
+#pragma unroll
+  for (int i = 0; i < kScoreLoads; ++i) w[i] = L::load(base, j0 + (int64_t)i * kScoreThreads * P, a.vocab);
+
+  float mine = kNegInf;
+#pragma unroll
+  for (int i = 0; i < kScoreLoads; ++i) {
+    float x[P];
+    L::unpack(w[i], x);
+#pragma unroll
+    for (int e = 0; e < P; ++e) mine = fmaxf(mine, x[e]);
+  }
+  const float m = block_reduce(mine, red, [](float p, float q) { return fmaxf(p, q); });
+  const float ref = m == kNegInf ? 0.f : m;
+  float s = 0.f, t = 0.f;
+#pragma unroll
+  for (int i = 0; i < kScoreLoads; ++i) {
+    float x[P];
+    L::unpack(w[i], x);
+#pragma unroll
+    for (int e = 0; e < P; ++e) {
+      const float d = x[e] - ref;
+      const float p = __builtin_amdgcn_exp2f(d * kLog2e);
+      s += p;
+      t = fmaf(p, fmaxf(d, kFarBelow), t);
+    }
+  }
+  const auto add = [](float p, float q) { return p + q; };
+  s = block_reduce(s, red, add);
+  t = block_reduce(t, red, add);
+
+  uint64_t* entries = nullptr;  // this chunk's top_k, sorted
+  if constexpr (TOP) {
+    __shared__ uint64_t found[kScoreCandidates];
+    __shared__ uint32_t quads[64];
+    __shared__ uint64_t keys[kScoreThreads / 64];
+    __shared__ int count;
+    const int k = a.top_k;
+    ScorePart* parts = (ScorePart*)a.workspace;
+    entries = (uint64_t*)(parts + a.rows * chunks) + (row * chunks + chunk) * (int64_t)k;
+    // A bound that at least k entries reach: the k-th largest of the maxima of
+    // 64 groups of four threads (k <= 32). Entries above it come from fewer
+    // than k groups.
+    uint32_t best = 0;
+#pragma unroll
+    for (int i = 0; i < kScoreLoads; ++i) {
+      float x[P];
+      L::unpack(w[i], x);
+#pragma unroll
+      for (int e = 0; e < P; ++e) {
+        const int64_t j = j0 + (int64_t)i * kScoreThreads * P + e;
+        const uint32_t o = j < a.vocab ? order_of(x[e]) : 0u;
+        best = best > o ? best : o;
+      }
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      const uint32_t other = __shfl_xor(best, o);
+      best = best > other ? best : other;
+    }
+    if (tid == 0) count = 0;
+    if ((tid & 3) == 0) quads[tid >> 2] = best;
+    __syncthreads();
+    if (tid < 64) {
+      const uint32_t q = quads[tid];
+      int above = 0;
+      for (int i = 0; i < 64; ++i) above += quads[i] > q || (quads[i] == q && i < tid);
+      if (above == k - 1) keys[0] = q;
+    }
+    __syncthreads();
+    const uint32_t bound = (uint32_t)keys[0];
+    __syncthreads();
+    if (bound != 0) {  // (0: fewer than k groups hold entries)
+#pragma unroll
+      for (int i = 0; i < kScoreLoads; ++i) {
+        float x[P];
+        L::unpack(w[i], x);
+#pragma unroll
+        for (int e = 0; e < P; ++e) {
+          const int64_t j = j0 + (int64_t)i * kScoreThreads * P + e;
+          if (j < a.vocab && order_of(x[e]) >= bound) {
+            const int at = atomicAdd(&count, 1);
+            if (at < kScoreCandidates) found[at] = entry_key(x[e], j);
+          }
+        }
+      }
+    }
+    __syncthreads();
+    const int n = count;
+    if (bound != 0 && n <= kScoreCandidates) {
+      // distinct keys: an entry's rank is the number of larger ones
+      for (int c = tid; c < n; c += kScoreThreads) {
+        const uint64_t key = found[c];
+        int rank = 0;
+        for (int i = 0; i < n; ++i) rank += found[i] > key;
+        if (rank < k) entries[rank] = key;
+      }
+    } else {
+      // many equal values (or a chunk of few): one entry at a time, the largest
+      // key below the last
+      uint64_t last = ~0ull;
+      for (int r = 0; r < k; ++r) {
+        uint64_t top = 0;
+#pragma unroll
+        for (int i = 0; i < kScoreLoads; ++i) {
+          float x[P];
+          L::unpack(w[i], x);
+#pragma unroll
+          for (int e = 0; e < P; ++e) {
+            const int64_t j = j0 + (int64_t)i * kScoreThreads * P + e;
+            const uint64_t key = j < a.vocab ? entry_key(x[e], j) : 0;
+            if (key < last && key > top) top = key;
+          }
+        }
+        top = block_reduce(top, keys, [](uint64_t p, uint64_t q) { return p > q ? p : q; });
+        if (tid == 0) entries[r] = top;  // 0: the chunk has no further entry
+        last = top;
+      }
+    }
+  }
+  if (tid == 0) {
+    if (chunks > 1 || TOP) ((ScorePart*)a.workspace)[row * chunks + chunk] = ScorePart{m, s, t, 0.f};
+    else finish_row(a, row, m, s, t, token_logit<DT>(a, base, row));
+  }
+}
+
+// One wave per row: the chunks' statistics and sorted entries merged.
+template <int DT>
+__global__ __launch_bounds__(64) void score_merge_kernel(const wmx_score_args a, int chunks) {
+  const int64_t row = blockIdx.x;
+  const int lane = threadIdx.x;
+  const ScorePart* parts = (const ScorePart*)a.workspace + row * chunks;
+  float m = kNegInf;
+  for (int c = lane; c < chunks; c += 64) m = fmaxf(m, parts[c].m);
+  m = wave_reduce(m, [](float p, float q) { return fmaxf(p, q); });
+  const float ref = m == kNegInf ? 0.f : m;
+  float s = 0.f, t = 0.f;
+  for (int c = lane; c < chunks; c += 64) {
+    const float d = parts[c].m - ref;
+    const float f = __builtin_amdgcn_exp2f(d * kLog2e);
+    s += parts[c].s * f;
+    t += f * (parts[c].t + parts[c].s * fmaxf(d, kFarBelow));
+  }
+  const auto add = [](float p, float q) { return p + q; };
+  s = wave_reduce(s, add);
+  t = wave_reduce(t, add);
+  const void* base = (const char*)a.logits + row * a.row_stride * Logit<DT>::kSize;
+  if (lane == 0) finish_row(a, row, m, s, t, token_logit<DT>(a, base, row));
+  const int k = a.top_k;
+  if (k == 0) return;
+  const uint64_t* entries = (const uint64_t*)((const ScorePart*)a.workspace + a.rows * chunks) + row * chunks * (int64_t)k;
+  const float log_s = logf(s);
+  const bool empty = m == kNegInf && s == 0.f;
+  // the next of all chunks' entries k times: the largest key below the last
+  uint64_t last = ~0ull;
+  for (int r = 0; r < k; ++r) {
+    uint64_t top = 0;
+    for (int i = lane; i < chunks * k; i += 64) {
+      const uint64_t key = entries[i];
+      if (key < last && key > top) top = key;
+    }
+    top = wave_reduce(top, [](uint64_t p, uint64_t q) { return p > q ? p : q; });
+    if (lane == 0) {
+      a.top_indices[row * k + r] = entry_index(top);
+      a.top_log_probs[row * k + r] = empty ? kNegInf : (value_of((uint32_t)(top >> 32)) - ref) - log_s;
+    }
+    last = top;
+  }
+}
+
+// The gradient: p (slope) for every logit of a chunk, then the chunk's few
+// named positions once more with what reaches their log probabilities.
+template <int DT>
+__global__ __launch_bounds__(kScoreThreads) void score_bwd_kernel(const wmx_score_args a, int chunks) {
+  using L = Logit<DT>;
+  constexpr int P = L::kPer;
+  const int64_t row = blockIdx.x / chunks;
+  const int chunk = (int)(blockIdx.x - row * chunks);
+  const int tid = threadIdx.x, k = a.top_k;
+  const void* base = (const char*)a.logits + row * a.row_stride * L::kSize;
+  void* out = (char*)a.grad_logits + row * (int64_t)a.vocab * L::kSize;
+  const int64_t begin = (int64_t)chunk * L::kChunk, j0 = begin + tid * P;
+
+  u32x4 w[kScoreLoads];
+#pragma unroll
+  for (int i = 0; i < kScoreLoads; ++i) w[i] = L::load(base, j0 + (int64_t)i * kScoreThreads * P, a.vocab);
+
+  const float lse = a.lse[row], entropy = a.entropy[row];
+  const int64_t token = a.tokens[row];
+  float g_token = a.grad_log_probs && token != a.ignore_index ? a.grad_log_probs[row] : 0.f;
+  if (token != a.ignore_index && (token < 0 || token >= a.vocab) && a.grad_log_probs) g_token = __builtin_nanf("");
+  const float g_entropy = a.grad_entropy ? a.grad_entropy[row] : 0.f;
+  float sum = g_token;
+  if (a.grad_top)
+    for (int i = 0; i < k; ++i) sum += a.grad_top[row * k + i];
+  const bool empty = lse == kNegInf;
+  const auto slope = [&](float x) {
+    const float d = x - lse;
+    const float p = __builtin_amdgcn_exp2f(d * kLog2e);
+    const float g = -p * fmaf(g_entropy, d + entropy, sum);
+    return empty || p == 0.f ? 0.f : g;
+  };
+#pragma unroll
+  for (int i = 0; i < kScoreLoads; ++i) {
+    const int64_t j = j0 + (int64_t)i * kScoreThreads * P;
+    if (j >= a.vocab) break;
+    float x[P];
+    L::unpack(w[i], x);
+#pragma unroll
+    for (int e = 0; e < P; ++e) x[e] = slope(x[e]);
+    if (j + P <= a.vocab) {
+      __builtin_nontemporal_store(L::pack(x), (u32x4_any*)((char*)out + j * L::kSize));
+    } else {
+#pragma unroll
+      for (int e = 0; e < P; ++e)
+        if (j + e < a.vocab) L::put(out, j + e, x[e]);
+    }
+  }
+  __builtin_amdgcn_s_waitcnt(0);  // the stores above have landed: the ones below replace some
+  __syncthreads();
+  if (tid > k || empty) return;
+  const int64_t at = tid == k ? (a.grad_log_probs && token != a.ignore_index ? token : -1)
+                              : (a.grad_top ? a.top_indices[row * k + tid] : -1);
+  if (at < begin || at >= begin + L::kChunk || at >= a.vocab) return;
+  float g = slope(L::one(base, at));
+  if (at == token) g += g_token;
+  if (a.grad_top)
+    for (int i = 0; i < k; ++i)
+      if (a.top_indices[row * k + i] == at) g += a.grad_top[row * k + i];
+  L::put(out, at, g);
+}
+
+template <int DT>
+int64_t score_chunks_of(const wmx_score_args& a) {
+  return ((int64_t)a.vocab + Logit<DT>::kChunk - 1) / Logit<DT>::kChunk;
+}
+static int64_t score_chunks(const wmx_score_args& a) {
+  return a.dtype == WMX_DTYPE_F32 ? score_chunks_of<WMX_DTYPE_F32>(a) : score_chunks_of<WMX_DTYPE_BF16>(a);
+}
+
+int64_t score_workspace_size(const wmx_score_args& a) {
+  return a.rows * score_chunks(a) * (int64_t)(sizeof(ScorePart) + a.top_k * sizeof(uint64_t));
+}
+
+template <int DT>
+static int launch_score_t(const wmx_score_args& a, hipStream_t stream) {
+  const int64_t chunks = score_chunks(a);
+  if (a.rows * chunks > INT32_MAX) return WMX_E_UNSUPPORTED;
+  const dim3 grid((unsigned)(a.rows * chunks));
+  if (a.top_k)
+    hipLaunchKernelGGL((score_kernel<DT, true>), grid, dim3(kScoreThreads), 0, stream, a, (int)chunks);
+  else
+    hipLaunchKernelGGL((score_kernel<DT, false>), grid, dim3(kScoreThreads), 0, stream, a, (int)chunks);
+  if (chunks > 1 || a.top_k)
+    hipLaunchKernelGGL((score_merge_kernel<DT>), dim3((unsigned)a.rows), dim3(64), 0, stream, a, (int)chunks);
+  return WMX_OK;
+}
+
+int launch_score(const wmx_score_args& a, hipStream_t stream) {
+  if (a.dtype == WMX_DTYPE_F32) return launch_score_t<WMX_DTYPE_F32>(a, stream);
+  if (a.dtype == WMX_DTYPE_BF16) return launch_score_t<WMX_DTYPE_BF16>(a, stream);
+  return launch_score_t<WMX_DTYPE_F16>(a, stream);
+}
+
+int launch_score_bwd(const wmx_score_args& a, hipStream_t stream) {
+  const int64_t chunks = score_chunks(a);
+  if (a.rows * chunks > INT32_MAX) return WMX_E_UNSUPPORTED;
+  const dim3 grid((unsigned)(a.rows * chunks));
+  if (a.dtype == WMX_DTYPE_F32)
+    hipLaunchKernelGGL((score_bwd_kernel<WMX_DTYPE_F32>), grid, dim3(kScoreThreads), 0, stream, a, (int)chunks);
+  else if (a.dtype == WMX_DTYPE_BF16)
+    hipLaunchKernelGGL((score_bwd_kernel<WMX_DTYPE_BF16>), grid, dim3(kScoreThreads), 0, stream, a, (int)chunks);
+  else
+    hipLaunchKernelGGL((score_bwd_kernel<WMX_DTYPE_F16>), grid, dim3(kScoreThreads), 0, stream, a, (int)chunks);
+  return WMX_OK;
+}
+
+}  // namespace wmx

@@ -36,40 +36,14 @@
 #include <utility>
 #include <vector>
 
-#include "wmx_attn.h"
+#include "torch_common.h"
 
 namespace {
 
 using at::Tensor;
+using namespace wmx_torch;
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
-
-// ------------------------------------------------------------ operands ----
-bool vector_ready(const Tensor& x) {
-  if (x.stride(-1) != 1 && x.size(-1) != 1) return false;
-  if (reinterpret_cast<uintptr_t>(x.data_ptr()) % 16) return false;
-  for (int64_t d = 0; d + 1 < x.dim(); ++d)
-    if (x.size(d) > 1 && x.stride(d) % 8) return false;
-  return true;
-}
-
-// bf16 with unit head_dim stride and 16-byte aligned rows; strided views
-// (cache channels, capacity padding, BQHD storage) are kept without a copy
-Tensor operand(Tensor x) {
-  if (x.scalar_type() != at::kBFloat16) x = x.to(at::kBFloat16);
-  if (vector_ready(x)) return x;
-  x = x.contiguous();
-  return vector_ready(x) ? x : x.clone();
-}
-
-// [batch, head, token] element strides of a 4-D tensor; size-1 dims give 0
-void strides3(const Tensor& x, int64_t (&out)[3]) {
-  for (int d = 0; d < 3; ++d) out[d] = x.size(d) > 1 ? x.stride(d) : 0;
-}
-
-void check_rc(int rc, const char* what) {
-  TORCH_CHECK(rc == WMX_OK, what, " failed (", rc, "): ", wmx_last_error());
-}
 
 void check_residue(int64_t stride, int64_t residue) {
   // residue -1 is the strict-past shift of residue 0
@@ -326,8 +300,6 @@ void fill_visibility(wmx_attn_args& a, const Schedule* s, const std::array<Tenso
     a.k_qend = either(s->docs[3], (*meta)[3]).data_ptr<int32_t>();
   }
 }
-
-hipStream_t stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
 std::tuple<Tensor, Tensor> forward_impl(const Tensor& Q, const Tensor& K, const Tensor& V,
                                         const std::array<Tensor, 4>* meta, int64_t stride, int64_t residue) {
@@ -746,11 +718,6 @@ c10::optional<Tensor> row_bounds(const c10::optional<Tensor>& t) {
   return t->contiguous();
 }
 
-Tensor mask_bytes(const c10::optional<Tensor>& key_mask) {
-  if (!key_mask) return Tensor();
-  return key_mask->contiguous().view(at::kByte);
-}
-
 constexpr int64_t kQueryTile = 128;
 
 std::tuple<Tensor, Tensor> strict_dense_fwd(const Tensor& query, const Tensor& key, const Tensor& value,
@@ -921,12 +888,6 @@ void strict_decode_out(const Tensor& out, const Tensor& query, const Tensor& key
 }
 
 // ------------------------------------------------- layer steps ----
-// Contiguous and 16-byte aligned.
-Tensor dense16(const Tensor& t) {
-  Tensor c = t.contiguous();
-  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 ? c.clone() : c;
-}
-
 // A norm's weight as the kernels read it: bfloat16, or float32 (the type that
 // the norm's arithmetic casts any other to).
 Tensor norm_weight(const Tensor& t) { return dense16(t.scalar_type() == at::kBFloat16 ? t : t.to(at::kFloat)); }

@@ -83,5 +83,13 @@ int64_t plan_workspace_size(const wmx_plan_args& a);
 int64_t plan_unit_workspace_size(const wmx_plan_args& a);
 int launch_plan_count(const wmx_plan_args& a, hipStream_t stream);
 int launch_plan_fill(const wmx_plan_args& a, hipStream_t stream);
+int launch_kv_quant(const wmx_kv_quant_args& a, hipStream_t stream);
+int launch_kv_read(const wmx_kv_read_args& a, hipStream_t stream);
+int tree_num_splits(const wmx_tree_args& a);
+int64_t tree_workspace_size(const wmx_tree_args& a);
+int launch_tree(const wmx_tree_args& a, hipStream_t stream);
+int64_t score_workspace_size(const wmx_score_args& a);
+int launch_score(const wmx_score_args& a, hipStream_t stream);
+int launch_score_bwd(const wmx_score_args& a, hipStream_t stream);
 
 }  // namespace wmx

@@ -27,14 +27,24 @@ when the keys are bf16. The in-place pool write is forward-only; training
 projects keys through `k_norm_rope`, an operator (white_matter::k_norm_rope)
 whose backward is one HIP kernel pair (wmx_kv_store_bwd: the key gradient
 and the norm weight's gradient summed in a fixed order).
+
+A pool may hold its rows quantised (`QuantizedPool`: e4m3 or int8 codes and one
+fp32 scale per row, about half the bytes): `write_pool_quantized` is the store
+into it, `quantize_pool` converts rows that are there already, `read_pool`
+reads them back as bf16, and `tree_attention` decodes over it.
 """
 
 from __future__ import annotations
+
+from typing import NamedTuple
 
 import torch
 import torch.nn.functional as F
 
 from . import _kernels, _native
+
+# kv_quant_store and kv_quant_read (csrc/serve_ops.cpp, kv_quant.hip)
+_native.load_ops()
 
 _DTYPES = {torch.float32: _native.DTYPE_F32, torch.bfloat16: _native.DTYPE_BF16}
 
@@ -120,6 +130,177 @@ def write_pool(
     a.batch, a.channels, a.heads, a.tokens, a.head_dim = batch, channels, heads, tokens, dim
     a.pool_slots, a.eps = keys.shape[3], float(eps)
     _native.kv_pool_store(a, key.device)
+
+
+# --------------------------------------------------------- quantised pool ----
+class QuantizedPool(NamedTuple):
+    """Pool rows as codes and scales: value = codes * scales[..., None].
+
+    codes (..., N, D) torch.float8_e4m3fn or torch.int8, scales (..., N)
+    float32. A row x is stored with scale = max|x| / T and code = x * (T /
+    max|x|) rounded to nearest even, T = 448 (e4m3) or 127 (int8); a row whose
+    largest magnitude is below 2^-100 as zeros with scale 0; a row that holds
+    an infinity or a NaN with scale NaN, so that it reads back as NaN.
+    """
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    @classmethod
+    def empty(
+        cls, shape: tuple[int, ...], *, dtype: torch.dtype = torch.float8_e4m3fn, device: torch.device | str = "cuda"
+    ) -> "QuantizedPool":
+        """A pool of zero rows of the given (..., N, D) shape."""
+        if dtype not in _CODE_DTYPES:
+            raise ValueError(f"a quantised pool holds float8_e4m3fn or int8 codes, not {dtype}")
+        codes = torch.zeros(shape, device=device, dtype=torch.uint8).view(dtype)
+        return cls(codes, torch.zeros(shape[:-1], device=device, dtype=torch.float32))
+
+    @property
+    def shape(self) -> torch.Size:
+        return self.codes.shape
+
+    @property
+    def device(self) -> torch.device:
+        return self.codes.device
+
+    @property
+    def dtype(self) -> torch.dtype:
+        return self.codes.dtype
+
+    def select(self, dim: int, index: int) -> "QuantizedPool":
+        """The view at `index` of a dimension before the slots (a channel)."""
+        if not 0 <= dim < self.codes.ndim - 2:
+            raise ValueError("select takes a dimension before the slots")
+        return QuantizedPool(self.codes.select(dim, index), self.scales.select(dim, index))
+
+
+_CODE_DTYPES = (torch.float8_e4m3fn, torch.int8)
+_HEAD_DIMS = (64, 96, 128)
+
+
+def _check_codes(pool: QuantizedPool, what: str, ndim: int = 5) -> None:
+    if not isinstance(pool, QuantizedPool):
+        raise TypeError(f"{what} must be a QuantizedPool, got {type(pool).__name__}")
+    codes, scales = pool
+    if codes.dtype not in _CODE_DTYPES or scales.dtype != torch.float32:
+        raise ValueError(f"{what} must hold float8_e4m3fn or int8 codes and float32 scales")
+    if codes.ndim != ndim or scales.shape != codes.shape[:-1] or scales.device != codes.device:
+        raise ValueError(f"{what} must hold codes of {ndim} dimensions and scales of the same shape without the last")
+    dim = codes.shape[-1]
+    if dim not in _HEAD_DIMS:
+        raise ValueError(f"head_dim {dim} is not supported (64, 96 or 128)")
+    if codes.stride(-1) != 1 or any(s % 8 for s, n in zip(codes.stride()[:-1], codes.shape) if n > 1):
+        raise ValueError("pool views need unit stride along D and aligned rows of codes")
+
+
+def _check_slots(slots: torch.Tensor, batch: int, what: str = "slots") -> None:
+    if slots.dtype not in (torch.int32, torch.int64) or slots.ndim not in (1, 2) or (slots.ndim == 2 and slots.shape[0] != batch):
+        raise ValueError(f"{what} must be integer (T,) or (B, T)")
+
+
+def write_pool_quantized(
+    key: torch.Tensor,
+    value: torch.Tensor | None,
+    k_norm_weight: torch.Tensor,
+    cos: torch.Tensor,
+    sin: torch.Tensor,
+    keys: QuantizedPool,
+    values: QuantizedPool | None,
+    slots: torch.Tensor,
+    *,
+    eps: float = 1e-6,
+    rope_by_slot: bool = False,
+) -> None:
+    """`write_pool` into a quantised pool: keys[:, :, :, slots] =
+    quantised(rope(rms_norm(key) * k_norm_weight)) and values[:, :, :, slots] =
+    quantised(value), in place, in one pass. The keys are computed in fp32 and
+    rounded once, as codes (`write_pool` rounds bf16 keys after every step).
+
+    key/value (B, C, H, T, D) float32 or bfloat16, k_norm_weight (C, D),
+    cos/sin (B, T, D), or (N, D) tables by slot with rope_by_slot, keys/values
+    pools (B, C, H, N, D) of one code type, or views of them. slots (T,), the
+    same for every batch row, or (B, T): the distinct slots of each row, whose
+    contents are otherwise undefined; a slot outside [0, N) is skipped. head_dim
+    64, 96 or 128.
+    """
+    _forward_only("write_pool_quantized", key, value, k_norm_weight, cos, sin)
+    if key.ndim != 5 or (value is not None and value.shape != key.shape):
+        raise ValueError("key and value must be (B, C, H, T, D) of one shape")
+    _dtype(key, "key"), _dtype(k_norm_weight, "k_norm_weight"), _dtype(cos, "cos")
+    if value is not None:
+        _dtype(value, "value")
+    batch, channels, heads, tokens, dim = key.shape
+    _check_codes(keys, "keys")
+    if (values is None) != (value is None):
+        raise ValueError("values must be given exactly when value is")
+    if keys.codes.shape[:3] != (batch, channels, heads) or keys.codes.shape[4] != dim:
+        raise ValueError("keys must be a (B, C, H, N, D) pool")
+    if values is not None:
+        _check_codes(values, "values")
+        if values.codes.shape != keys.codes.shape or values.codes.dtype != keys.codes.dtype:
+            raise ValueError("values must be a pool of the keys' shape and code type")
+    if k_norm_weight.shape != (channels, dim):
+        raise ValueError("k_norm_weight must be (C, D)")
+    if rope_by_slot:
+        if cos.shape != (keys.codes.shape[3], dim) or sin.shape != cos.shape or sin.dtype != cos.dtype:
+            raise ValueError("with rope_by_slot, cos and sin must be (N, D) tables of one dtype")
+    elif cos.shape != (batch, tokens, dim) or sin.shape != cos.shape or sin.dtype != cos.dtype:
+        raise ValueError("cos and sin must be (B, T, D) of one dtype")
+    _check_slots(slots, batch)
+    if slots.shape[-1] != tokens:
+        raise ValueError("slots must be (T,) or (B, T)")
+    _on_gpu("write_pool_quantized", key)
+    torch.ops.white_matter.kv_quant_store(
+        key, value, k_norm_weight, cos, sin, slots, keys.codes, keys.scales, None if values is None else values.codes,
+        None if values is None else values.scales, rope_by_slot, float(eps),
+    )
+
+
+def quantize_pool(rows: torch.Tensor, dtype: torch.dtype = torch.float8_e4m3fn) -> QuantizedPool:
+    """A new quantised pool of the given rows (B, C, H, N, D) float32 or
+    bfloat16: what `write_pool` wrote during a prefill, for a decode over it."""
+    _forward_only("quantize_pool", rows)
+    if dtype not in _CODE_DTYPES:
+        raise ValueError(f"a quantised pool holds float8_e4m3fn or int8 codes, not {dtype}")
+    if rows.ndim != 5 or rows.shape[-1] not in _HEAD_DIMS:
+        raise ValueError("rows must be (B, C, H, N, D) with head_dim 64, 96 or 128")
+    _dtype(rows, "rows")
+    _on_gpu("quantize_pool", rows)
+    codes = torch.empty(rows.shape, device=rows.device, dtype=dtype)
+    scales = torch.empty(rows.shape[:-1], device=rows.device, dtype=torch.float32)
+    torch.ops.white_matter.kv_quant_store(None, rows, None, None, None, None, None, None, codes, scales, False, 0.0)
+    return QuantizedPool(codes, scales)
+
+
+def read_pool(pool: QuantizedPool, slots: torch.Tensor | None = None) -> torch.Tensor:
+    """bf16(codes * scales) of a quantised pool (B, C, H, N, D): every slot, or
+    slots (T,) or (B, T) (one list per batch row) in their order, as a new
+    (B, C, H, T, D) tensor. A slot outside [0, N) reads as zeros."""
+    _check_codes(pool, "pool")
+    if slots is not None:
+        _check_slots(slots, pool.codes.shape[0])
+    _on_gpu("read_pool", pool.codes)
+    return torch.ops.white_matter.kv_quant_read(pool.codes, pool.scales, slots)
+
+
+def _forward_only(name: str, *tensors: torch.Tensor | None) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{name} is forward-only")
+
+
+def _on_gpu(name: str, t: torch.Tensor) -> None:
+    if not t.is_cuda:
+        raise RuntimeError(f"{name} runs on the HIP kernels: it takes GPU tensors")
+
+
+torch.library.register_fake("white_matter::kv_quant_store", lambda *args: None)
+
+
+@torch.library.register_fake("white_matter::kv_quant_read")
+def _(codes, scales, slots):
+    tokens = codes.shape[3] if slots is None else slots.shape[-1]
+    return codes.new_empty((*codes.shape[:3], tokens, codes.shape[4]), dtype=torch.bfloat16)
 
 
 @torch.library.custom_op("white_matter::k_norm_rope", mutates_args=())

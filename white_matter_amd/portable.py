@@ -90,3 +90,47 @@ def strict_causal_attention_portable(
     read = keep.any(1)[:, None, :, None]
     key, value = key.masked_fill(~read, 0), value.masked_fill(~read, 0)
     return _math_sdpa(query, key, value, keep[:, None], scale).transpose(1, 2)
+
+
+def tree_attention_portable(query, key, value, key_scales, value_scales, kv_lengths, tree_mask, use_dummy_token, key_mask, scale):
+    batch, heads, nodes, dim = query.shape
+    slots = key.shape[2]
+    if key_scales is not None:
+        key, value = key.float() * key_scales[..., None], value.float() * value_scales[..., None]
+    lengths = torch.as_tensor(kv_lengths, device=query.device).long().expand(batch).clamp_min(0)
+    node = torch.arange(slots, device=query.device) - (lengths + int(use_dummy_token))[:, None, None]  # (B, 1, N)
+    keep = (node < 0).expand(batch, nodes, slots)
+    if tree_mask is not None:
+        at = node.clamp(0, max(nodes - 1, 0)).expand(batch, nodes, slots)
+        keep = keep | ((node >= 0) & (node < nodes) & tree_mask.expand(batch, nodes, nodes).gather(2, at))
+    if key_mask is not None:
+        keep = keep & key_mask[:, None, :]
+    # float32 products, one query at a time's weights against the values it
+    # sees: a slot that one query must not see may hold anything
+    q = query.float().unflatten(1, (key.shape[1], -1))  # (B, Hkv, G, n, D)
+    k, v = key.float(), value.float()
+    scores = torch.matmul(q, k[:, :, None].transpose(-1, -2)) * scale
+    scores = scores.masked_fill(~keep[:, None, None], float("-inf"))
+    weight = torch.softmax(scores, -1).masked_fill(~keep.any(-1)[:, None, None, :, None], 0.0)
+    odd = ~torch.isfinite(v)
+    out = torch.matmul(weight, v.masked_fill(odd, 0.0)[:, :, None])
+    if bool(odd.any()):
+        weight = weight.masked_fill(~keep[:, None, None], 0.0)
+        seen = keep[:, None, None, :, :, None] & odd[:, :, None, None]
+        out = out + torch.where(seen, weight[..., None] * v[:, :, None, None], 0.0).sum(-2)
+    return out.flatten(1, 2).transpose(1, 2).to(query.dtype)
+
+
+def token_log_probs_portable(logits, tokens, top_k, ignore_index):
+    x = logits.float()
+    most = x.amax(-1, keepdim=True)
+    empty = most == float("-inf")
+    logp = torch.log_softmax(x.masked_fill(empty, 0.0), -1).masked_fill(empty, float("-inf"))
+    p = logp.exp()
+    entropy = -(p * logp.masked_fill(p == 0, 0.0)).sum(-1)
+    ignored = tokens == ignore_index
+    outside = ((tokens < 0) | (tokens >= x.shape[-1])) & ~ignored
+    log_probs = logp.gather(-1, tokens.clamp(0, x.shape[-1] - 1)[..., None])[..., 0]
+    log_probs = log_probs.masked_fill(outside, float("nan")).masked_fill(ignored, 0.0)
+    indices = torch.sort(x.detach(), dim=-1, descending=True, stable=True).indices[..., :top_k]
+    return log_probs, entropy, logp.gather(-1, indices), indices
