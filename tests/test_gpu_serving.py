@@ -218,7 +218,7 @@ def _pool_pair(gen, shape, kind):
 
 @pytest.mark.parametrize("kind", ["bf16", "e4m3", "int8"])
 @pytest.mark.parametrize("dim", [64, 96, 128])
-@pytest.mark.parametrize(("heads", "kv_heads", "nodes"), [(4, 4, 1), (6, 2, 5), (4, 2, 13), (8, 2, 11), (10, 2, 16)])
+@pytest.mark.parametrize(("heads", "kv_heads", "nodes"), [(4, 4, 1), (6, 2, 5), (4, 2, 13), (8, 2, 11), (10, 2, 13), (8, 2, 16), (10, 2, 16)])
 @pytest.mark.parametrize("splits", [0, 1, 3])
 @torch.no_grad()
 def test_tree_attention(kind, dim, heads, kv_heads, nodes, splits):

@@ -165,7 +165,7 @@ def test_pool_refusals():
         (dict(value=key), ValueError, "exactly when"),
         (dict(values=pool), ValueError, "exactly when"),
         (dict(keys=key), TypeError, "QuantizedPool"),
-        (dict(keys=_pool(heads=3)), ValueError, "keys must be"),
+        (dict(keys=_pool(heads=3)), ValueError, "B, C, H, N, D"),
         (dict(value=key, values=_pool(dtype=torch.int8)), ValueError, "code type"),
         (dict(weight=torch.ones(2, 64)), ValueError, "k_norm_weight"),
         (dict(cos=torch.ones(2, 4, 64)), ValueError, "cos and sin"),
@@ -183,7 +183,7 @@ def test_pool_refusals():
     wide = _pool(dim=128)
     with pytest.raises(ValueError, match="unit stride"):
         kv_pool.read_pool(kv_pool.QuantizedPool(wide.codes[..., ::2], wide.scales))
-    for shape, message in (((2, 1, 2, 3, 80), "head_dim"), ((2, 2, 3, 64), "B, C, H, N, D")):
+    for shape, message in (((2, 1, 2, 3, 80), "head_dim"), ((2, 2, 3, 64), "B, C, H, T, D")):
         with pytest.raises(ValueError, match=message):
             kv_pool.quantize_pool(torch.zeros(shape))
     with pytest.raises(ValueError, match="codes"):

@@ -749,9 +749,11 @@ int wmx_tree_attn(const wmx_tree_args* a, void* stream) {
   for (const int64_t* st : {a->k_stride, a->v_stride}) {
     for (int i = 0; i < 3; ++i)
       if (st[i] % unit) return fail(WMX_E_INVALID, "pool rows must be 16-byte aligned");
-    if (st[2] < 0 || st[2] * (codes ? 1 : 2) >= (1 << 25))
-      return fail(WMX_E_UNSUPPORTED, "pool slots must lie less than 2^25 bytes apart");
+    if (st[2] != 0 && (st[2] < a->head_dim || st[2] * (codes ? 1 : 2) >= (1 << 25)))
+      return fail(WMX_E_UNSUPPORTED, "pool slots must lie at least head_dim elements and less than 2^25 bytes apart");
   }
+  if (a->tree_mask && (a->tree_mask_stride[1] < 0 || a->tree_mask_stride[1] * (int64_t)a->nodes > INT32_MAX - a->nodes))
+    return fail(WMX_E_UNSUPPORTED, "a row's tree mask spans 2^31 bytes");
   const int64_t need = wmx::tree_workspace_size(*a);
   if (need > 0 && (!a->workspace || a->workspace_bytes < need || !aligned16(a->workspace)))
     return fail(WMX_E_WORKSPACE, "tree attention needs %lld workspace bytes", (long long)need);

@@ -61,12 +61,13 @@ __device__ __forceinline__ u32x2 quantise_row(float (&x)[8], float& scale) {
 
 // One (b, c, t, head group) per L consecutive lanes (token-fastest, so
 // neighbouring lanes read and write neighbouring rows); each thread walks its
-// group's heads, U at a time with all their loads issued before any is used.
-template <int D, int FMT, bool KEY, bool ROPE, bool VALUE>
+// group's heads, U at a time with all their loads issued before any is used (a
+// group of one head takes U = 1: the others repeat their last head instead of
+// testing).
+template <int D, int FMT, int U, bool KEY, bool ROPE, bool VALUE>
 __global__ __launch_bounds__(256) void kv_quant_kernel(const wmx_kv_quant_args a, int64_t tokens_total, int head_groups) {
   constexpr int LD = D / 8;           // lanes holding data
   constexpr int L = LD <= 8 ? 8 : 16; // lanes per row (a power of two; D = 96 leaves 4 idle)
-  constexpr int U = 4;                // heads in flight per thread
   const int64_t gid = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   const int64_t unit = gid / L;
   const int l = (int)(gid % L);
@@ -161,19 +162,25 @@ __global__ __launch_bounds__(256) void kv_quant_kernel(const wmx_kv_quant_args a
   }
 }
 
-template <int D, int FMT>
-static void launch_kv_quant_d(const wmx_kv_quant_args& a, int64_t rows, int groups, dim3 grid, hipStream_t stream) {
+template <int D, int FMT, int U>
+static void launch_kv_quant_u(const wmx_kv_quant_args& a, int64_t rows, int groups, dim3 grid, hipStream_t stream) {
   const bool rope = a.k_norm_weight != nullptr;
   if (!a.key)
-    hipLaunchKernelGGL((kv_quant_kernel<D, FMT, false, false, true>), grid, dim3(256), 0, stream, a, rows, groups);
+    hipLaunchKernelGGL((kv_quant_kernel<D, FMT, U, false, false, true>), grid, dim3(256), 0, stream, a, rows, groups);
   else if (rope && a.value)
-    hipLaunchKernelGGL((kv_quant_kernel<D, FMT, true, true, true>), grid, dim3(256), 0, stream, a, rows, groups);
+    hipLaunchKernelGGL((kv_quant_kernel<D, FMT, U, true, true, true>), grid, dim3(256), 0, stream, a, rows, groups);
   else if (rope)
-    hipLaunchKernelGGL((kv_quant_kernel<D, FMT, true, true, false>), grid, dim3(256), 0, stream, a, rows, groups);
+    hipLaunchKernelGGL((kv_quant_kernel<D, FMT, U, true, true, false>), grid, dim3(256), 0, stream, a, rows, groups);
   else if (a.value)
-    hipLaunchKernelGGL((kv_quant_kernel<D, FMT, true, false, true>), grid, dim3(256), 0, stream, a, rows, groups);
+    hipLaunchKernelGGL((kv_quant_kernel<D, FMT, U, true, false, true>), grid, dim3(256), 0, stream, a, rows, groups);
   else
-    hipLaunchKernelGGL((kv_quant_kernel<D, FMT, true, false, false>), grid, dim3(256), 0, stream, a, rows, groups);
+    hipLaunchKernelGGL((kv_quant_kernel<D, FMT, U, true, false, false>), grid, dim3(256), 0, stream, a, rows, groups);
+}
+
+template <int D, int FMT>
+static void launch_kv_quant_d(const wmx_kv_quant_args& a, int64_t rows, int groups, dim3 grid, hipStream_t stream) {
+  if (groups == a.heads) launch_kv_quant_u<D, FMT, 1>(a, rows, groups, grid, stream);
+  else launch_kv_quant_u<D, FMT, 4>(a, rows, groups, grid, stream);
 }
 
 int launch_kv_quant(const wmx_kv_quant_args& a, hipStream_t stream) {

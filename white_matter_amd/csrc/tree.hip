@@ -18,7 +18,8 @@
 //                  consecutive d per lane and transposed between registers
 //                  (v_perm), so output block c holds d = (D/16) i + c
 // K and V scales multiply scores and weights, one operation per score instead
-// of one per element; codes are converted exactly to bf16.
+// of one per element. Codes are converted exactly: K's to bf16 like the
+// queries; V's to fp16, in which the weights keep 11 bits (bf16 pools: 8).
 #include <climits>
 
 #include "wmx_kernels.h"
@@ -26,14 +27,26 @@
 namespace wmx {
 
 constexpr int kTreeWaves = 4;
-constexpr int kTreeTile = 32;                          // slots per wave and step
-constexpr int kTreeStep = kTreeWaves * kTreeTile;      // slots per workgroup and step
+constexpr int kTreeTile = 32;                      // slots per wave and step
+constexpr int kTreeStep = kTreeWaves * kTreeTile;  // slots per workgroup and step
+// The running maximum follows a larger score only once it is past it by this
+// many powers of two: weights up to 2^8 cost no precision, and most steps
+// rescale nothing.
+constexpr float kLazyMax = 8.f;
+// V scales are multiplied by a power of two that keeps them at most 64, so that
+// weights times scales stay below 2^14 in fp16 (largest 65,504).
+constexpr float kScaleRoom = 64.f;
 
 __device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a), as_bf16x8(b), c, 0, 0, 0);
 }
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+__device__ __forceinline__ f32x4 mfma16_half(const u32x4& a, const u32x4& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
 
-// Two codes (the low or high half of a dword) as a bf16 pair, exactly.
+// Two codes (the low or high half of a dword) as a bf16 or fp16 pair, exactly.
 template <int FMT, bool HIGH>
 __device__ __forceinline__ uint32_t code_pair(uint32_t w) {
   if constexpr (FMT == WMX_POOL_E4M3) {
@@ -43,11 +56,33 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t w) {
     return pack_bf16x2((float)(int8_t)(w >> s), (float)(int8_t)(w >> (s + 8)));
   }
 }
+template <int FMT, bool HIGH>
+__device__ __forceinline__ uint32_t code_pair_half(uint32_t w) {
+  if constexpr (FMT == WMX_POOL_E4M3) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.0f, HIGH));
+  } else {
+    // 1024 + (code + 128) has the code's bits as its lowest: no conversion
+    const uint32_t biased = __builtin_amdgcn_perm(0x64646464u, w ^ 0x80808080u, HIGH ? 0x04030402u : 0x04010400u);
+    const f16x2 x = __builtin_bit_cast(f16x2, biased) - f16x2{(_Float16)1152.f, (_Float16)1152.f};
+    return __builtin_bit_cast(uint32_t, x);
+  }
+}
+
+typedef __amdgpu_buffer_rsrc_t tree_rsrc;
+// A raw buffer over [base, base + bytes), both wave-uniform; reads past it give zeros.
+__device__ __forceinline__ tree_rsrc tree_buffer(const char* base, int bytes) {
+  const uint64_t p = (uint64_t)base;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)p), hi = __builtin_amdgcn_readfirstlane((uint32_t)(p >> 32));
+  return __builtin_amdgcn_make_buffer_rsrc((void*)(((uint64_t)hi << 32) | lo), (short)0, __builtin_amdgcn_readfirstlane(bytes),
+                                           0x00020000);
+}
+constexpr int kReadOnce = 2;  // cache policy: nontemporal
 
 // How a wave reads 32 slots of K and V.
 template <int FMT, int D>
 struct TreeTile {
   static constexpr int kElem = FMT == WMX_POOL_BF16 ? 2 : 1;  // bytes
+  static constexpr int kRow = D * kElem;
   static constexpr int KS = D / 32;                           // k-steps of S^T
   static constexpr int W = D / 16;                            // consecutive d per lane of V
   // A lane's K operand of k-step s: bf16 and D = 96 codes take 8 d at
@@ -64,20 +99,19 @@ struct TreeTile {
     if constexpr (FMT != WMX_POOL_BF16 && D == 96) return c < 4 ? 4 * i + c : 64 + 2 * i + (c - 4);
     else return W * i + c;
   }
+  // the lane's key e of a tile
+  static __device__ __forceinline__ int key_of(int q, int e) { return 4 * q + (e & 3) + 16 * (e >> 2); }
 
   uint32_t k[2][KS][KD];  // key halves
-  uint32_t v[8][VD];      // the lane's keys: 4 q + (e & 3) + 16 (e >> 2)
+  uint32_t v[8][VD];      // the lane's keys
 
-  // lk(row), lv(row): byte offset of a tile row from the (wave-uniform) base
-  template <class Row>
-  __device__ __forceinline__ void load_k(const char* base, int li, int q, Row row) {
+  __device__ __forceinline__ void load_k(const tree_rsrc& rs, const int (&off)[2]) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const char* p = base + row(16 * u + li);
       if constexpr (kWide) {
 #pragma unroll
         for (int j = 0; j < KS / 2; ++j) {
-          const u32x4 w = __builtin_nontemporal_load((const u32x4*)(p + 16 * (q + 4 * j)));
+          const auto w = __builtin_amdgcn_raw_buffer_load_b128(rs, off[u] + 64 * j, 0, kReadOnce);
 #pragma unroll
           for (int i = 0; i < 4; ++i) k[u][2 * j + i / 2][i % 2] = w[i];
         }
@@ -85,11 +119,11 @@ struct TreeTile {
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
           if constexpr (FMT == WMX_POOL_BF16) {
-            const u32x4 w = __builtin_nontemporal_load((const u32x4*)(p + 16 * (q + 4 * s)));
+            const auto w = __builtin_amdgcn_raw_buffer_load_b128(rs, off[u] + 64 * s, 0, kReadOnce);
 #pragma unroll
             for (int i = 0; i < 4; ++i) k[u][s][i] = w[i];
           } else {
-            const u32x2 w = __builtin_nontemporal_load((const u32x2*)(p + 8 * (q + 4 * s)));
+            const auto w = __builtin_amdgcn_raw_buffer_load_b64(rs, off[u] + 32 * s, 0, kReadOnce);
             k[u][s][0] = w[0];
             k[u][s][1] = w[1];
           }
@@ -97,35 +131,35 @@ struct TreeTile {
       }
     }
   }
-  template <class Row>
-  __device__ __forceinline__ void load_v(const char* base, int li, int q, Row row) {
-    typedef u32x4 u32x4_4 __attribute__((aligned(4)));
-    typedef uint32_t u32x3 __attribute__((ext_vector_type(3)));
-    typedef u32x3 u32x3_4 __attribute__((aligned(4)));
-    typedef u32x2 u32x2_4 __attribute__((aligned(4)));
+  // byte offset of the lane's K part in a row
+  static __device__ __forceinline__ int k_part(int q) { return kWide || FMT == WMX_POOL_BF16 ? 16 * q : 8 * q; }
+
+  __device__ __forceinline__ void load_v(const tree_rsrc& rs, const int (&off)[8], int li) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const char* p = base + row(4 * q + (e & 3) + 16 * (e >> 2));
       if constexpr (FMT != WMX_POOL_BF16 && D == 96) {
-        v[e][0] = __builtin_nontemporal_load((const uint32_t*)(p + 4 * li));
-        v[e][1] = __builtin_nontemporal_load((const uint16_t*)(p + 64 + 2 * li));
+        v[e][0] = __builtin_amdgcn_raw_buffer_load_b32(rs, off[e], 0, kReadOnce);
+        v[e][1] = __builtin_amdgcn_raw_buffer_load_b16(rs, off[e] + 64 - 2 * li, 0, kReadOnce);
       } else if constexpr (VD == 4) {
-        const u32x4 w = __builtin_nontemporal_load((const u32x4_4*)(p + 16 * li));
+        const auto w = __builtin_amdgcn_raw_buffer_load_b128(rs, off[e], 0, kReadOnce);
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[e][i] = w[i];
       } else if constexpr (VD == 3) {
-        const u32x3 w = __builtin_nontemporal_load((const u32x3_4*)(p + 12 * li));
+        const auto w = __builtin_amdgcn_raw_buffer_load_b96(rs, off[e], 0, kReadOnce);
 #pragma unroll
         for (int i = 0; i < 3; ++i) v[e][i] = w[i];
       } else if constexpr (VD == 2) {
-        const u32x2 w = __builtin_nontemporal_load((const u32x2_4*)(p + 8 * li));
+        const auto w = __builtin_amdgcn_raw_buffer_load_b64(rs, off[e], 0, kReadOnce);
         v[e][0] = w[0];
         v[e][1] = w[1];
       } else {
-        v[e][0] = __builtin_nontemporal_load((const uint32_t*)(p + 4 * li));
+        v[e][0] = __builtin_amdgcn_raw_buffer_load_b32(rs, off[e], 0, kReadOnce);
       }
     }
   }
+  // byte offset of the lane's V part in a row (its first part, D = 96 codes)
+  static __device__ __forceinline__ int v_part(int li) { return FMT != WMX_POOL_BF16 && D == 96 ? 4 * li : W * kElem * li; }
+
   // MFMA operand of key half u, k-step s
   __device__ __forceinline__ u32x4 k_operand(int u, int s) const {
     if constexpr (FMT == WMX_POOL_BF16) {
@@ -135,12 +169,18 @@ struct TreeTile {
                    code_pair<FMT, true>(k[u][s][1])};
     }
   }
-  // bf16 pair w (elements 2 w, 2 w + 1 of the lane's W) of key e
+  // pair w (elements 2 w, 2 w + 1 of the lane's W) of key e: bf16, or fp16 of codes
   __device__ __forceinline__ uint32_t v_pair(int e, int w) const {
     if constexpr (FMT == WMX_POOL_BF16) return v[e][w];
-    else return w & 1 ? code_pair<FMT, true>(v[e][w / 2]) : code_pair<FMT, false>(v[e][w / 2]);
+    else return w & 1 ? code_pair_half<FMT, true>(v[e][w / 2]) : code_pair_half<FMT, false>(v[e][w / 2]);
   }
+  // exponent bits of a value that is not finite, in a v_pair's low half
+  static constexpr uint32_t kOdd = FMT == WMX_POOL_BF16 ? 0x7f80u : 0x7c00u;
 };
+
+// A value as if it changed here: what is derived from it (the lane masks of its
+// bits, a pair of scalar registers each) is formed at its use and not kept.
+__device__ __forceinline__ void fresh(uint32_t& x) { __asm__ volatile("" : "+v"(x)); }
 
 struct TreeRange {
   int base;   // committed slots (every node sees them)
@@ -157,18 +197,261 @@ __device__ __forceinline__ TreeRange tree_range(const wmx_tree_args& a, int b) {
   return TreeRange{__builtin_amdgcn_readfirstlane((int)base), __builtin_amdgcn_readfirstlane((int)total)};
 }
 
-__device__ __forceinline__ float lane_from(float x, int lane) {
-  return __uint_as_float(__builtin_amdgcn_ds_bpermute(lane << 2, __float_as_uint(x)));
+// x of lanes l ^ 16 and l ^ 32 joined with this lane's, the same in all four
+__device__ __forceinline__ float max_quarters(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return max_halves(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float sum_quarters(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return sum_halves(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
+// One wave's state over its tiles, every kTreeWaves-th of its workgroup's.
 template <int FMT, int D, int MB>
-__global__ __launch_bounds__(64 * kTreeWaves, MB == 4 ? 1 : 2) void tree_kernel(const wmx_tree_args a, int units, int tiles,
+struct TreeWave {
+  using Tile = TreeTile<FMT, D>;
+  static constexpr int KS = Tile::KS, W = Tile::W;
+
+  u32x4 qf[MB][KS];  // queries, the B operand
+  float m[MB], l[MB];
+  f32x4 acc[MB][W];
+  float vref;        // V scales are multiplied by it (a power of two)
+  Tile tile;
+  float ks[8], vs[8];
+  int koff[2], voff[8];
+  uint32_t kept[8];  // key_mask of the lane's keys
+  bool odd;          // this lane met a drafted value that is not finite
+
+  // of the whole wave
+  const char *kbase, *vbase;
+  const float *kscale, *vscale;
+  const uint8_t *kmask, *tmask;
+  int node_at[MB];                   // offset of this lane's node's row in tmask
+  int tree_bytes;
+  int64_t ksb, vsb;                  // bytes between slots
+  int base, end;
+  float scale;
+
+  static __device__ __forceinline__ int span(int slots, int64_t step) {
+    return (int)((min(slots, kTreeTile) - 1) * step) + Tile::kRow;
+  }
+  __device__ __forceinline__ void load_scales(int j0, const float* src, int q, float (&out)[8]) {
+    if constexpr (FMT != WMX_POOL_BF16) {
+      typedef f32x4 f32x4_4 __attribute__((aligned(4)));
+      if (j0 + kTreeTile <= end) {
+        const f32x4 a = *(const f32x4_4*)(src + j0 + 4 * q), b = *(const f32x4_4*)(src + j0 + 16 + 4 * q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          out[e] = a[e];
+          out[4 + e] = b[e];
+        }
+      } else {  // the last slot's for those behind it, which are masked
+#pragma unroll
+        for (int e = 0; e < 8; ++e) out[e] = src[min(j0 + Tile::key_of(q, e), end - 1)];
+      }
+    }
+  }
+  // slots past the last visible one read as zeros
+  template <bool EDGE>
+  __device__ __forceinline__ void load_k(int j0, int q) {
+    tile.load_k(tree_buffer(kbase + j0 * ksb, span(end - j0, ksb)), koff);
+    load_scales(j0, kscale, q, ks);
+    if (EDGE && kmask) {  // (zero past the last slot; with a key mask every tile is an edge)
+      const tree_rsrc rs = tree_buffer((const char*)kmask, end);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) kept[e] = __builtin_amdgcn_raw_buffer_load_b8(rs, j0 + Tile::key_of(q, e), 0, 0);
+    }
+  }
+  __device__ __forceinline__ void load_v(int j0, int q, int li) {
+    tile.load_v(tree_buffer(vbase + j0 * vsb, span(end - j0, vsb)), voff, li);
+    load_scales(j0, vscale, q, vs);
+  }
+
+  // One tile. EDGE: some of its slots are masked, drafted or past the end.
+  template <bool EDGE>
+  __device__ __forceinline__ void step(int j0, int li, int q) {
+    uint32_t seen[MB];      // bit e: this lane's query sees its key e
+    uint32_t keep[8];       // 0: no query may see key e, else all ones
+    uint32_t drafted = 0u;  // bit e: key e is a drafted one
+    const bool any_drafted = EDGE && j0 + kTreeTile > base && end > base;
+    if constexpr (EDGE) {
+      uint32_t kept_bits = 0u;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int j = j0 + Tile::key_of(q, e);
+        const bool ok = j < end && (!kmask || kept[e] != 0);
+        keep[e] = ok ? ~0u : 0u;
+        fresh(keep[e]);
+        kept_bits |= (ok ? 1u : 0u) << e;
+        drafted |= (ok && j >= base ? 1u : 0u) << e;
+      }
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) seen[mb] = kept_bits;
+      if (any_drafted) {
+        // (a query's bytes past the last slot and before the first drafted one are not read)
+        const tree_rsrc rs = tree_buffer((const char*)tmask, tree_bytes);
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
+          uint32_t t[8];
+          fresh(drafted);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const int a = j0 + Tile::key_of(q, e) - base;
+            t[e] = __builtin_amdgcn_raw_buffer_load_b8(rs, (drafted >> e) & 1u ? node_at[mb] + a : -1, 0, 0);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) seen[mb] &= ~((t[e] ? 0u : (drafted >> e) & 1u) << e);
+        }
+      }
+    }
+    float sc[MB][8];
+    {
+      f32x4 s[MB][2];
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) s[mb][0] = s[mb][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int st = 0; st < KS; ++st) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const u32x4 kf = tile.k_operand(u, st);
+#pragma unroll
+          for (int mb = 0; mb < MB; ++mb) s[mb][u] = mfma16(kf, qf[mb][st], s[mb][u]);
+        }
+      }
+      float kq[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) kq[e] = FMT == WMX_POOL_BF16 ? scale : scale * ks[e];
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sc[mb][e] = s[mb][e >> 2][e & 3] * kq[e];
+      }
+    }
+    const int next = j0 + kTreeStep;
+    if (next < end) load_k<EDGE>(next, q);  // K's registers are free
+
+    if constexpr (EDGE) {
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) {
+        fresh(seen[mb]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sc[mb][e] = (seen[mb] >> e) & 1u ? sc[mb][e] : kNegInf;
+      }
+    }
+
+    if constexpr (FMT != WMX_POOL_BF16) {
+      float most = 0.f;  // (NaN stays out of it, and an infinity)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) most = fmaxf(most, vs[e] < kPosInf ? vs[e] : 0.f);
+      if (__any(most * vref > kScaleRoom)) {
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o));
+        const int up = 132 - (int)(__float_as_uint(most) >> 23);  // most * 2^up in [32, 64)
+        const float ref = __uint_as_float((uint32_t)(127 + min(up, 120)) << 23);
+        const float f = ref / vref;
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) {
+#pragma unroll
+          for (int c = 0; c < W; ++c) acc[mb][c] *= f;
+        }
+        vref = ref;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) vs[e] *= vref;
+    }
+
+    u32x4 p[MB];  // weights (times V scales), the B operand
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+      float top = fmaxf(sc[mb][0], sc[mb][1]);
+#pragma unroll
+      for (int e = 2; e < 8; ++e) top = fmaxf(top, sc[mb][e]);
+      if (__any(top > m[mb] + kLazyMax)) {
+        const float mn = fmaxf(m[mb], max_quarters(top));
+        const float f = mn == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m[mb] - mn);
+        l[mb] *= f;
+#pragma unroll
+        for (int c = 0; c < W; ++c) acc[mb][c] *= f;
+        m[mb] = mn;
+      }
+      const float ref = m[mb] == kNegInf ? 0.f : m[mb];
+      float x[8];
+      if constexpr (EDGE) fresh(seen[mb]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = __builtin_amdgcn_exp2f(sc[mb][e] - ref);
+        l[mb] += x[e];
+        if constexpr (FMT != WMX_POOL_BF16) {
+          x[e] *= vs[e];
+          if constexpr (EDGE) x[e] = (seen[mb] >> e) & 1u ? x[e] : 0.f;  // a masked row's scale may be NaN
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (FMT == WMX_POOL_BF16) {
+          p[mb][i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+        } else {
+          const f16x2 h = {(_Float16)x[2 * i], (_Float16)x[2 * i + 1]};
+          p[mb][i] = __builtin_bit_cast(uint32_t, h);
+        }
+      }
+    }
+
+    // O^T += V^T P^T, output blocks 2 w and 2 w + 1 at a time
+#pragma unroll
+    for (int w = 0; w < W / 2; ++w) {
+      uint32_t x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = tile.v_pair(e, w);
+      if constexpr (EDGE && FMT != WMX_POOL_INT8) {
+        // Zero times an infinity is no zero: masked rows leave the product, and
+        // so do the values of drafted rows that are not finite, since some
+        // queries do not see them (the others get them with the output).
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] &= keep[e];
+        if (any_drafted) {
+          fresh(drafted);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const bool draft = (drafted >> e) & 1u;
+            const bool lo = draft && (x[e] & Tile::kOdd) == Tile::kOdd;
+            const bool hi = draft && (x[e] & (Tile::kOdd << 16)) == Tile::kOdd << 16;
+            odd |= lo || hi;
+            x[e] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
+          }
+        }
+      }
+      u32x4 v0, v1;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v0[i] = __builtin_amdgcn_perm(x[2 * i + 1], x[2 * i], 0x05040100u);
+        v1[i] = __builtin_amdgcn_perm(x[2 * i + 1], x[2 * i], 0x07060302u);
+      }
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) {
+        if constexpr (FMT == WMX_POOL_BF16) {
+          acc[mb][2 * w] = mfma16(v0, p[mb], acc[mb][2 * w]);
+          acc[mb][2 * w + 1] = mfma16(v1, p[mb], acc[mb][2 * w + 1]);
+        } else {
+          acc[mb][2 * w] = mfma16_half(v0, p[mb], acc[mb][2 * w]);
+          acc[mb][2 * w + 1] = mfma16_half(v1, p[mb], acc[mb][2 * w + 1]);
+        }
+      }
+    }
+    if (next < end) load_v(next, q, li);
+  }
+};
+
+template <int FMT, int D, int MB>
+__global__ __launch_bounds__(64 * kTreeWaves, (MB == 1 && TreeTile<FMT, D>::kRow < 256) ? 3 : 2) void tree_kernel(const wmx_tree_args a, int units, int tiles,
                                                                           int nsplit, int chunk) {
   using Tile = TreeTile<FMT, D>;
   constexpr int KS = Tile::KS, W = Tile::W, ROWS = 16 * MB;
   constexpr int LDR = 4 * W + 4;  // LDS row of one merge round: four quarters x W, padded against bank conflicts
   __shared__ __attribute__((aligned(16))) float lds_o[kTreeWaves][ROWS][LDR];
-  __shared__ float lds_m[kTreeWaves][ROWS], lds_l[kTreeWaves][ROWS];
+  __shared__ float lds_m[kTreeWaves][ROWS], lds_l[kTreeWaves][ROWS], lds_max[ROWS], lds_sum[ROWS];
+  __shared__ int lds_odd;
 
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
   const int li = lane & 15, q = lane >> 4;
@@ -185,251 +468,109 @@ __global__ __launch_bounds__(64 * kTreeWaves, MB == 4 ? 1 : 2) void tree_kernel(
 
   const TreeRange range = tree_range(a, b);
   const int begin = split * chunk, end = min(begin + chunk, range.total);
-  const float scale = a.softmax_scale * kLog2e;
+  const uint8_t* kmask = a.key_mask ? a.key_mask + (int64_t)b * a.key_mask_stride : nullptr;
+  const uint8_t* tmask = a.tree_mask ? a.tree_mask + (int64_t)b * a.tree_mask_stride[0] : nullptr;
+  const char* vbase = (const char*)a.v + ((int64_t)b * a.v_stride[0] + (int64_t)hk * a.v_stride[1]) * Tile::kElem;
+  const int64_t vsb = a.v_stride[2] * Tile::kElem;
+  if (tid == 0) lds_odd = 0;
 
-  float m[MB], l[MB];
-  f32x4 acc[MB][W];
+  TreeWave<FMT, D, MB> w;
+  w.vref = 0x1p120f;
+  w.odd = false;
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) {
-    m[mb] = kNegInf;
-    l[mb] = 0.f;
+    w.m[mb] = kNegInf;
+    w.l[mb] = 0.f;
 #pragma unroll
-    for (int c = 0; c < W; ++c) acc[mb][c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int c = 0; c < W; ++c) w.acc[mb][c] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  if (begin < end) {
+  int j0 = begin + kTreeTile * wave;
+  if (j0 < end) {
+    w.kbase = (const char*)a.k + ((int64_t)b * a.k_stride[0] + (int64_t)hk * a.k_stride[1]) * Tile::kElem;
+    w.vbase = vbase;
+    w.ksb = a.k_stride[2] * Tile::kElem;
+    w.vsb = vsb;
+    if constexpr (FMT != WMX_POOL_BF16) {
+      w.kscale = a.k_scales + (int64_t)b * a.k_scales_stride[0] + (int64_t)hk * a.k_scales_stride[1];
+      w.vscale = a.v_scales + (int64_t)b * a.v_scales_stride[0] + (int64_t)hk * a.v_scales_stride[1];
+    }
+    w.kmask = kmask;
+    w.tmask = tmask;
+    w.tree_bytes = (int)((a.nodes - 1) * a.tree_mask_stride[1]) + a.nodes;
+    w.base = range.base;
+    w.end = end;
+    w.scale = a.softmax_scale * kLog2e;
+#pragma unroll
+    for (int u = 0; u < 2; ++u) w.koff[u] = (16 * u + li) * (int)w.ksb + Tile::k_part(q);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) w.voff[e] = Tile::key_of(q, e) * (int)vsb + Tile::v_part(li);
+    w.template load_k<true>(j0, q);
+    w.load_v(j0, q, li);
     // this lane's queries: rows row0 + 16 mb + li (zeros past the last)
-    u32x4 qf[MB][KS];
-    int node[MB];
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) {
       const int r = row0 + 16 * mb + li;
       const bool ok = r < rows;
       const int i = ok ? r / group : 0, h = hk * group + (ok ? r - i * group : 0);
-      node[mb] = i;
+      w.node_at[mb] = i * (int)a.tree_mask_stride[1];
       const bf16* p = (const bf16*)a.q + (int64_t)b * a.q_stride[0] + (int64_t)h * a.q_stride[1] + (int64_t)i * a.q_stride[2];
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        const u32x4 w = load16(p + Tile::k_dim(s, q));
+        const u32x4 x = load16(p + Tile::k_dim(s, q));
         const u32x4 z = {0u, 0u, 0u, 0u};
-        qf[mb][s] = ok ? w : z;
+        w.qf[mb][s] = ok ? x : z;
       }
     }
-    const char* kbase = (const char*)a.k + ((int64_t)b * a.k_stride[0] + (int64_t)hk * a.k_stride[1]) * Tile::kElem;
-    const char* vbase = (const char*)a.v + ((int64_t)b * a.v_stride[0] + (int64_t)hk * a.v_stride[1]) * Tile::kElem;
-    const int64_t ksb = a.k_stride[2] * Tile::kElem, vsb = a.v_stride[2] * Tile::kElem;
-    const float* kscale = FMT == WMX_POOL_BF16 ? nullptr : a.k_scales + (int64_t)b * a.k_scales_stride[0] + (int64_t)hk * a.k_scales_stride[1];
-    const float* vscale = FMT == WMX_POOL_BF16 ? nullptr : a.v_scales + (int64_t)b * a.v_scales_stride[0] + (int64_t)hk * a.v_scales_stride[1];
-    const uint8_t* kmask = a.key_mask ? a.key_mask + (int64_t)b * a.key_mask_stride : nullptr;
-    const uint8_t* tmask = a.tree_mask ? a.tree_mask + (int64_t)b * a.tree_mask_stride[0] : nullptr;
-    const int ks32 = (int)ksb, vs32 = (int)vsb;  // a tile's rows span less than 2^31 bytes (checked on the host)
-
-    Tile tile;
-    float ks[8], vs[8];  // scales of the lane's keys
-    const auto load_scales = [&](int j0, int last, const float* src, float (&out)[8]) {
-      if constexpr (FMT != WMX_POOL_BF16) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) out[e] = src[j0 + min(4 * q + (e & 3) + 16 * (e >> 2), last)];
-      }
-    };
-    // rows past the last visible slot are read as the last one and masked
-    const auto load_k = [&](int j0) {
-      const int last = end - 1 - j0;
-      tile.load_k(kbase + j0 * ksb, li, q, [&](int row) { return min(row, last) * ks32; });
-      load_scales(j0, last, kscale, ks);
-    };
-    const auto load_v = [&](int j0) {
-      const int last = end - 1 - j0;
-      tile.load_v(vbase + j0 * vsb, li, q, [&](int row) { return min(row, last) * vs32; });
-      load_scales(j0, last, vscale, vs);
-    };
-
-    int j0 = begin + kTreeTile * wave;
-    if (j0 < end) {
-      load_k(j0);
-      load_v(j0);
-    }
-    for (; j0 < end; j0 += kTreeStep) {
-      // S^T = K Q^T
-      f32x4 s[MB][2];
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb) s[mb][0] = s[mb][1] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int st = 0; st < KS; ++st) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const u32x4 kf = tile.k_operand(u, st);
-#pragma unroll
-          for (int mb = 0; mb < MB; ++mb) s[mb][u] = mfma16(kf, qf[mb][st], s[mb][u]);
-        }
-      }
-      float sc[MB][8];
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          sc[mb][e] = s[mb][e >> 2][e & 3] * (FMT == WMX_POOL_BF16 ? scale : scale * ks[e]);
-      }
-      const int next = j0 + kTreeStep;
-      if (next < end) load_k(next);  // K's registers are free
-
-      // slots that some row does not see: past the committed ones, or masked
-      const bool edge = kmask || j0 + kTreeTile > min(range.base, end);
-      uint32_t seen[MB];  // bit e: this lane's query sees its key e
-      if (edge) {
-#pragma unroll
-        for (int mb = 0; mb < MB; ++mb) seen[mb] = 0u;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const int j = j0 + 4 * q + (e & 3) + 16 * (e >> 2);
-          bool ok = j < end;
-          if (ok && kmask) ok = kmask[j] != 0;
-#pragma unroll
-          for (int mb = 0; mb < MB; ++mb) {
-            bool vis = ok;
-            if (ok && j >= range.base) vis = tmask[(int64_t)node[mb] * a.tree_mask_stride[1] + (j - range.base)] != 0;
-            seen[mb] |= (vis ? 1u : 0u) << e;
-            sc[mb][e] = vis ? sc[mb][e] : kNegInf;
-          }
-        }
-      }
-
-      uint32_t p[MB][4];  // weights times V scales, the B operand
-      float pf[MB][8];
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb) {
-        float top = sc[mb][0];
-#pragma unroll
-        for (int e = 1; e < 8; ++e) top = fmaxf(top, sc[mb][e]);
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        if (__any(top > m[mb])) {
-          const float mn = fmaxf(m[mb], top);
-          const float f = mn == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m[mb] - mn);
-          l[mb] *= f;
-#pragma unroll
-          for (int c = 0; c < W; ++c) acc[mb][c] *= f;
-          m[mb] = mn;
-        }
-        const float ref = m[mb] == kNegInf ? 0.f : m[mb];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float w = __builtin_amdgcn_exp2f(sc[mb][e] - ref);
-          l[mb] += w;
-          float x = w;
-          if constexpr (FMT != WMX_POOL_BF16) {
-            x = w * vs[e];
-            if (edge) x = (seen[mb] >> e) & 1u ? x : 0.f;  // a masked row's scale may be NaN
-          }
-          pf[mb][e] = x;
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[mb][i] = pack_bf16x2(pf[mb][2 * i], pf[mb][2 * i + 1]);
-      }
-
-      // O^T += V^T P^T, output blocks 2 w and 2 w + 1 at a time
-      uint32_t odd = 0u;  // bit e: key e of this lane holds a value that is not finite
-#pragma unroll
-      for (int w = 0; w < W / 2; ++w) {
-        uint32_t x[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = tile.v_pair(e, w);
-        if (FMT != WMX_POOL_INT8 && edge) {
-          // A value that some row must not see may be anything: 0 times an
-          // infinity is no zero, so such values leave the product and are
-          // added below to the rows that see them.
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const bool lo = (x[e] & 0x7f80u) == 0x7f80u, hi = (x[e] & 0x7f800000u) == 0x7f800000u;
-            odd |= (lo || hi ? 1u : 0u) << e;
-            x[e] &= (lo ? 0u : 0xffffu) | (hi ? 0u : 0xffff0000u);
-          }
-        }
-        u32x4 v0, v1;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v0[i] = __builtin_amdgcn_perm(x[2 * i + 1], x[2 * i], 0x05040100u);
-          v1[i] = __builtin_amdgcn_perm(x[2 * i + 1], x[2 * i], 0x07060302u);
-        }
-#pragma unroll
-        for (int mb = 0; mb < MB; ++mb) {
-          const u32x4 pb = {p[mb][0], p[mb][1], p[mb][2], p[mb][3]};
-          acc[mb][2 * w] = mfma16(v0, pb, acc[mb][2 * w]);
-          acc[mb][2 * w + 1] = mfma16(v1, pb, acc[mb][2 * w + 1]);
-        }
-      }
-      if (FMT != WMX_POOL_INT8 && edge && __any(odd)) {
-        // key by key: the weight from the lane that holds it, the values from
-        // the lanes that loaded them
-#pragma unroll 1
-        for (int kq = 0; kq < 4; ++kq) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            if (!__any(q == kq && ((odd >> e) & 1u))) continue;
-#pragma unroll
-            for (int w = 0; w < W / 2; ++w) {
-              const uint32_t pair_bits = tile.v_pair(e, w);
-#pragma unroll
-              for (int r = 0; r < 4; ++r) {
-                const uint32_t bits = (uint32_t)__builtin_amdgcn_ds_bpermute((16 * kq + 4 * q + r) << 2, (int)pair_bits);
-#pragma unroll
-                for (int mb = 0; mb < MB; ++mb) {
-                  const float pw = lane_from(pf[mb][e], 16 * kq + li);
-                  const bool vis = (__builtin_amdgcn_ds_bpermute((16 * kq + li) << 2, (int)seen[mb]) >> e) & 1;
-                  const float lo = bf16_lo(bits), hi = bf16_hi(bits);
-                  if (vis && (bits & 0x7f80u) == 0x7f80u) acc[mb][2 * w][r] += pw * lo;
-                  if (vis && (bits & 0x7f800000u) == 0x7f800000u) acc[mb][2 * w + 1][r] += pw * hi;
-                }
-              }
-            }
-          }
-        }
-      }
-      if (next < end) load_v(next);
-    }
+    const int whole = kmask ? begin : min(range.base, end);  // slots that every query sees end here
+    for (; j0 + kTreeTile <= whole; j0 += kTreeStep) w.template step<false>(j0, li, q);
+    for (; j0 < end; j0 += kTreeStep) w.template step<true>(j0, li, q);
   }
 
   // the workgroup's waves merged: maxima and sums, then the outputs in four
   // rounds (round r: block rows 4 q + r, W consecutive d per lane)
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) {
-    l[mb] += __shfl_xor(l[mb], 16);
-    l[mb] += __shfl_xor(l[mb], 32);
+    w.l[mb] = sum_quarters(w.l[mb]);
     if (q == 0) {
-      lds_m[wave][16 * mb + li] = m[mb];
-      lds_l[wave][16 * mb + li] = l[mb];
+      lds_m[wave][16 * mb + li] = w.m[mb];
+      lds_l[wave][16 * mb + li] = w.l[mb];
     }
   }
   __syncthreads();
+  if (w.odd) lds_odd = 1;
   float* ws_o = (float*)a.workspace;
   float* ws_ml = ws_o + (int64_t)a.batch * a.q_heads * a.nodes * nsplit * D;
   const int64_t prow0 = ((int64_t)pair * rows + row0) * nsplit + split;  // partial of row row0; rows are nsplit apart
-  const auto row_max = [&](int row) {
-    float mx = lds_m[0][row];
+  // per row: the maximum over the waves, and what the outputs are divided by
+  if (tid < ROWS) {
+    float mx = lds_m[0][tid], sum = 0.f;
 #pragma unroll
-    for (int w = 1; w < kTreeWaves; ++w) mx = fmaxf(mx, lds_m[w][row]);
-    return mx;
-  };
-  const auto row_sum = [&](int row, float mx) {
-    float sum = 0.f;
+    for (int i = 1; i < kTreeWaves; ++i) mx = fmaxf(mx, lds_m[i][tid]);
 #pragma unroll
-    for (int w = 0; w < kTreeWaves; ++w)
-      if (lds_m[w][row] != kNegInf || lds_l[w][row] != 0.f) sum += lds_l[w][row] * __builtin_amdgcn_exp2f(lds_m[w][row] - mx);
-    return sum;
-  };
-  if (nsplit > 1 && tid < ROWS && row0 + tid < rows) {
-    const float mx = row_max(tid);
+    for (int i = 0; i < kTreeWaves; ++i) {
+      // (a wave that saw nothing has the sum 0, a row of NaN scores no maximum)
+      const float f = lds_m[i][tid] == kNegInf ? 1.f : __builtin_amdgcn_exp2f(lds_m[i][tid] - mx);
+      sum += lds_l[i][tid] == 0.f ? 0.f : lds_l[i][tid] * f;
+    }
+    lds_max[tid] = mx;
+    lds_sum[tid] = sum;
+  }
+  __syncthreads();
+  if (nsplit > 1 && tid < min(ROWS, rows - row0)) {
     float* out = ws_ml + (prow0 + (int64_t)tid * nsplit) * 2;
-    out[0] = mx;
-    out[1] = row_sum(tid, mx == kNegInf ? 0.f : mx);
+    out[0] = lds_max[tid];
+    out[1] = lds_sum[tid];
   }
   if (nsplit > 1 && begin >= end) return;  // (the workgroup agrees) its sum is zero: the merge skips it
   float factor[MB];  // this wave's share of its rows
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) {
-    const float mx = row_max(16 * mb + li);
-    factor[mb] = m[mb] == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m[mb] - mx);
-    if (m[mb] == kNegInf && l[mb] != 0.f) factor[mb] = 1.f;  // (a row of NaN scores)
+    const int row = 16 * mb + li;
+    const float f = w.m[mb] == kNegInf ? 1.f : __builtin_amdgcn_exp2f(w.m[mb] - lds_max[row]);
+    const float sum = nsplit > 1 ? 1.f : lds_sum[row];
+    factor[mb] = sum == 0.f ? 0.f : f / sum;
+    if constexpr (FMT != WMX_POOL_BF16) factor[mb] *= 1.f / w.vref;
   }
   constexpr int PAIRS = ROWS * 4 * W / 2;  // output pairs of a round
 #pragma unroll
@@ -440,8 +581,8 @@ __global__ __launch_bounds__(64 * kTreeWaves, MB == 4 ? 1 : 2) void tree_kernel(
 #pragma unroll
       for (int c = 0; c < W; c += 2) {
         float* dst = &lds_o[wave][16 * mb + li][W * q + c];
-        dst[0] = acc[mb][c][r] * factor[mb];
-        dst[1] = acc[mb][c + 1][r] * factor[mb];
+        dst[0] = w.acc[mb][c][r] * factor[mb];
+        dst[1] = w.acc[mb][c + 1][r] * factor[mb];
       }
     }
     __syncthreads();
@@ -451,27 +592,45 @@ __global__ __launch_bounds__(64 * kTreeWaves, MB == 4 ? 1 : 2) void tree_kernel(
       if (row0 + row >= rows) continue;
       float o0 = 0.f, o1 = 0.f;
 #pragma unroll
-      for (int w = 0; w < kTreeWaves; ++w) {
-        o0 += lds_o[w][row][W * qq + c];
-        o1 += lds_o[w][row][W * qq + c + 1];
+      for (int i4 = 0; i4 < kTreeWaves; ++i4) {
+        o0 += lds_o[i4][row][W * qq + c];
+        o1 += lds_o[i4][row][W * qq + c + 1];
       }
       const int d = Tile::v_dim(4 * qq + r, c);  // (c even: d and d + 1)
+      const int n = (row0 + row) / group, h = hk * group + (row0 + row - n * group);
+      if (FMT != WMX_POOL_INT8 && lds_odd) {
+        // drafted values that are not finite, for the queries that see them:
+        // any positive weight leaves them as they are
+        for (int j = max(begin, range.base); j < end; ++j) {
+          if (!tmask[(int64_t)n * a.tree_mask_stride[1] + (j - range.base)] || (kmask && !kmask[j])) continue;
+          const char* at = vbase + j * vsb + d * Tile::kElem;
+          float v0, v1;
+          if constexpr (FMT == WMX_POOL_BF16) {
+            v0 = bf16_lo(*(const uint32_t*)at);
+            v1 = bf16_hi(*(const uint32_t*)at);
+          } else {  // (only NaN)
+            const uint32_t u = *(const uint16_t*)at;
+            v0 = (u & 0x7fu) == 0x7fu ? __builtin_nanf("") : 0.f;
+            v1 = (u & 0x7f00u) == 0x7f00u ? __builtin_nanf("") : 0.f;
+          }
+          o0 += __builtin_isfinite(v0) ? 0.f : v0;
+          o1 += __builtin_isfinite(v1) ? 0.f : v1;
+        }
+      }
       if (nsplit > 1) {
         float* out = ws_o + (prow0 + (int64_t)row * nsplit) * D + d;
         out[0] = o0;
         out[1] = o1;
       } else {
-        const float mx = row_max(row), sum = row_sum(row, mx == kNegInf ? 0.f : mx);
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        const int n = (row0 + row) / group, h = hk * group + (row0 + row - n * group);
         bf16* out = (bf16*)a.o + (int64_t)b * a.o_stride[0] + (int64_t)h * a.o_stride[1] + (int64_t)n * a.o_stride[2] + d;
-        *(uint32_t*)out = pack_bf16x2(o0 * inv, o1 * inv);
+        *(uint32_t*)out = pack_bf16x2(o0, o1);
       }
     }
   }
 }
 
-// Merge of a row's ranges: one thread per four consecutive d.
+// Merge of a row's ranges: one thread per four consecutive d, eight ranges'
+// loads in flight.
 __global__ __launch_bounds__(256) void tree_merge_kernel(const wmx_tree_args a, int nsplit, int64_t threads) {
   const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (gid >= threads) return;
@@ -479,21 +638,34 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const wmx_tree_args a, 
   const int64_t row = gid / per;
   const int d = 4 * (int)(gid - row * per);
   const float* ws_o = (const float*)a.workspace;
-  const float* ws_ml = ws_o + (int64_t)a.batch * a.q_heads * a.nodes * nsplit * D + row * nsplit * 2;
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const f32x2* ws_ml = (const f32x2*)(ws_o + (int64_t)a.batch * a.q_heads * a.nodes * nsplit * D) + row * nsplit;
   ws_o += row * nsplit * D + d;
-  float mx = kNegInf;
-  for (int s = 0; s < nsplit; ++s) mx = fmaxf(mx, ws_ml[2 * s]);
-  const float ref = mx == kNegInf ? 0.f : mx;
-  float sum = 0.f;
+  float mx = kNegInf, sum = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int s = 0; s < nsplit; ++s) {
-    const float ls = ws_ml[2 * s + 1];
-    if (ls == 0.f) continue;  // an empty range wrote no output
-    const float ms = ws_ml[2 * s];
-    const float w = ms == kNegInf ? 1.f : __builtin_amdgcn_exp2f(ms - ref);
-    sum += ls * w;
-    const f32x4 part = *(const f32x4*)(ws_o + (int64_t)s * D);
-    o += part * w;
+  for (int s0 = 0; s0 < nsplit; s0 += 8) {
+    f32x2 ml[8];
+    f32x4 part[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      const int s = min(s0 + u, nsplit - 1);
+      ml[u] = ws_ml[s];
+      part[u] = *(const f32x4*)(ws_o + (int64_t)s * D);  // an empty range wrote none: not used
+    }
+    float top = mx;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) top = fmaxf(top, ml[u][0]);
+    const float f = mx == kNegInf ? 1.f : __builtin_amdgcn_exp2f(mx - top);  // (nothing to scale before a first maximum)
+    sum *= f;
+    o *= f;
+    mx = top;
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+      if (s0 + u >= nsplit || ml[u][1] == 0.f) continue;
+      const float w = ml[u][0] == kNegInf ? 1.f : __builtin_amdgcn_exp2f(ml[u][0] - top);
+      sum += ml[u][1] * w;
+      o += part[u] * w;
+    }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   const int64_t pair = row / rows;
@@ -505,22 +677,22 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const wmx_tree_args a, 
   *(u32x2_4*)out = w;
 }
 
-// Query rows per workgroup, in 16s.
-static int tree_blocks(const wmx_tree_args& a) {
-  const int64_t rows = (int64_t)a.nodes * (a.q_heads / a.kv_heads);
-  return rows <= 16 ? 1 : rows <= 32 ? 2 : 4;
-}
-static int64_t tree_tiles(const wmx_tree_args& a) {
+// Query rows per workgroup in 16s. Two 16s use 240 registers, two waves a SIMD;
+// three and four share the conversions further but leave one wave a SIMD
+// (measured: 64 nodes x 2 heads over 16 x 8,192 slots 128 us with two, 167 with
+// four, 194 with three).
+static int tree_blocks(const wmx_tree_args& a) { return (int64_t)a.nodes * (a.q_heads / a.kv_heads) <= 16 ? 1 : 2; }
+static int64_t tree_workgroups(const wmx_tree_args& a) {  // per key range
   const int64_t rows = (int64_t)a.nodes * (a.q_heads / a.kv_heads), per = 16 * tree_blocks(a);
-  return (rows + per - 1) / per;
+  return (rows + per - 1) / per * a.batch * a.kv_heads;
 }
 
 int tree_num_splits(const wmx_tree_args& a) {
   if (a.num_splits > 0) return a.num_splits;
-  const int64_t wgs = (int64_t)a.batch * a.kv_heads * tree_tiles(a);
+  const int64_t wgs = tree_workgroups(a);
   if (wgs <= 0) return 1;
   int64_t splits = (4 * 256 + wgs - 1) / wgs;
-  const int64_t most = ((int64_t)a.capacity + 2 * kTreeStep - 1) / (2 * kTreeStep);
+  const int64_t most = ((int64_t)a.capacity + 255) / 256;
   if (splits > most) splits = most;
   return splits < 1 ? 1 : (int)splits;
 }
@@ -530,29 +702,32 @@ int64_t tree_workspace_size(const wmx_tree_args& a) {
   return s == 1 ? 0 : (int64_t)a.batch * a.q_heads * a.nodes * s * (a.head_dim + 2) * (int64_t)sizeof(float);
 }
 
+struct TreeLaunch {
+  int units, tiles, nsplit, chunk;
+};
+
 template <int FMT, int D>
-static void launch_tree_d(const wmx_tree_args& a, unsigned blocks, int units, int tiles, int nsplit, int chunk, hipStream_t stream) {
+static void launch_tree_d(const wmx_tree_args& a, unsigned blocks, const TreeLaunch& t, hipStream_t stream) {
   const dim3 grid(blocks), block(64 * kTreeWaves);
-  switch (tree_blocks(a)) {
-    case 1: hipLaunchKernelGGL((tree_kernel<FMT, D, 1>), grid, block, 0, stream, a, units, tiles, nsplit, chunk); break;
-    case 2: hipLaunchKernelGGL((tree_kernel<FMT, D, 2>), grid, block, 0, stream, a, units, tiles, nsplit, chunk); break;
-    default: hipLaunchKernelGGL((tree_kernel<FMT, D, 4>), grid, block, 0, stream, a, units, tiles, nsplit, chunk); break;
-  }
+  if (tree_blocks(a) == 1)
+    hipLaunchKernelGGL((tree_kernel<FMT, D, 1>), grid, block, 0, stream, a, t.units, t.tiles, t.nsplit, t.chunk);
+  else
+    hipLaunchKernelGGL((tree_kernel<FMT, D, 2>), grid, block, 0, stream, a, t.units, t.tiles, t.nsplit, t.chunk);
 }
 
 template <int FMT>
-static int launch_tree_f(const wmx_tree_args& a, unsigned blocks, int units, int tiles, int nsplit, int chunk, hipStream_t stream) {
+static int launch_tree_f(const wmx_tree_args& a, unsigned blocks, const TreeLaunch& t, hipStream_t stream) {
   switch (a.head_dim) {
-    case 64: launch_tree_d<FMT, 64>(a, blocks, units, tiles, nsplit, chunk, stream); return WMX_OK;
-    case 96: launch_tree_d<FMT, 96>(a, blocks, units, tiles, nsplit, chunk, stream); return WMX_OK;
-    case 128: launch_tree_d<FMT, 128>(a, blocks, units, tiles, nsplit, chunk, stream); return WMX_OK;
+    case 64: launch_tree_d<FMT, 64>(a, blocks, t, stream); return WMX_OK;
+    case 96: launch_tree_d<FMT, 96>(a, blocks, t, stream); return WMX_OK;
+    case 128: launch_tree_d<FMT, 128>(a, blocks, t, stream); return WMX_OK;
     default: return WMX_E_UNSUPPORTED;
   }
 }
 
 int launch_tree(const wmx_tree_args& a, hipStream_t stream) {
   const int nsplit = tree_num_splits(a);
-  const int64_t units = (int64_t)nsplit * a.batch * a.kv_heads, tiles = tree_tiles(a);
+  const int64_t pairs = (int64_t)a.batch * a.kv_heads, units = nsplit * pairs, tiles = tree_workgroups(a) / pairs;
   const int64_t blocks = (units + 7) / 8 * 8 * tiles;
   const int64_t merged = (int64_t)a.batch * a.q_heads * a.nodes * (a.head_dim / 4);
   if (blocks > INT32_MAX || (merged + 255) / 256 > INT32_MAX) return WMX_E_UNSUPPORTED;
@@ -560,10 +735,11 @@ int launch_tree(const wmx_tree_args& a, hipStream_t stream) {
   chunk = (chunk + kTreeStep - 1) / kTreeStep * kTreeStep;
   if (chunk < kTreeStep) chunk = kTreeStep;
   if (chunk * nsplit > INT32_MAX) return WMX_E_UNSUPPORTED;  // (ranges begin within 31 bits)
+  const TreeLaunch t{(int)units, (int)tiles, nsplit, (int)chunk};
   int rc;
-  if (a.format == WMX_POOL_BF16) rc = launch_tree_f<WMX_POOL_BF16>(a, (unsigned)blocks, (int)units, (int)tiles, nsplit, (int)chunk, stream);
-  else if (a.format == WMX_POOL_E4M3) rc = launch_tree_f<WMX_POOL_E4M3>(a, (unsigned)blocks, (int)units, (int)tiles, nsplit, (int)chunk, stream);
-  else rc = launch_tree_f<WMX_POOL_INT8>(a, (unsigned)blocks, (int)units, (int)tiles, nsplit, (int)chunk, stream);
+  if (a.format == WMX_POOL_BF16) rc = launch_tree_f<WMX_POOL_BF16>(a, (unsigned)blocks, t, stream);
+  else if (a.format == WMX_POOL_E4M3) rc = launch_tree_f<WMX_POOL_E4M3>(a, (unsigned)blocks, t, stream);
+  else rc = launch_tree_f<WMX_POOL_INT8>(a, (unsigned)blocks, t, stream);
   if (rc != WMX_OK || nsplit == 1) return rc;
   hipLaunchKernelGGL(tree_merge_kernel, dim3((unsigned)((merged + 255) / 256)), dim3(256), 0, stream, a, nsplit, merged);
   return WMX_OK;

@@ -176,27 +176,14 @@ class QuantizedPool(NamedTuple):
 
 
 _CODE_DTYPES = (torch.float8_e4m3fn, torch.int8)
-_HEAD_DIMS = (64, 96, 128)
 
 
-def _check_codes(pool: QuantizedPool, what: str, ndim: int = 5) -> None:
+def _parts(pool: QuantizedPool | None, what: str) -> tuple[torch.Tensor | None, torch.Tensor | None]:
+    if pool is None:
+        return None, None
     if not isinstance(pool, QuantizedPool):
         raise TypeError(f"{what} must be a QuantizedPool, got {type(pool).__name__}")
-    codes, scales = pool
-    if codes.dtype not in _CODE_DTYPES or scales.dtype != torch.float32:
-        raise ValueError(f"{what} must hold float8_e4m3fn or int8 codes and float32 scales")
-    if codes.ndim != ndim or scales.shape != codes.shape[:-1] or scales.device != codes.device:
-        raise ValueError(f"{what} must hold codes of {ndim} dimensions and scales of the same shape without the last")
-    dim = codes.shape[-1]
-    if dim not in _HEAD_DIMS:
-        raise ValueError(f"head_dim {dim} is not supported (64, 96 or 128)")
-    if codes.stride(-1) != 1 or any(s % 8 for s, n in zip(codes.stride()[:-1], codes.shape) if n > 1):
-        raise ValueError("pool views need unit stride along D and aligned rows of codes")
-
-
-def _check_slots(slots: torch.Tensor, batch: int, what: str = "slots") -> None:
-    if slots.dtype not in (torch.int32, torch.int64) or slots.ndim not in (1, 2) or (slots.ndim == 2 and slots.shape[0] != batch):
-        raise ValueError(f"{what} must be integer (T,) or (B, T)")
+    return pool.codes, pool.scales
 
 
 def write_pool_quantized(
@@ -224,52 +211,22 @@ def write_pool_quantized(
     contents are otherwise undefined; a slot outside [0, N) is skipped. head_dim
     64, 96 or 128.
     """
-    _forward_only("write_pool_quantized", key, value, k_norm_weight, cos, sin)
-    if key.ndim != 5 or (value is not None and value.shape != key.shape):
-        raise ValueError("key and value must be (B, C, H, T, D) of one shape")
-    _dtype(key, "key"), _dtype(k_norm_weight, "k_norm_weight"), _dtype(cos, "cos")
-    if value is not None:
-        _dtype(value, "value")
-    batch, channels, heads, tokens, dim = key.shape
-    _check_codes(keys, "keys")
-    if (values is None) != (value is None):
-        raise ValueError("values must be given exactly when value is")
-    if keys.codes.shape[:3] != (batch, channels, heads) or keys.codes.shape[4] != dim:
-        raise ValueError("keys must be a (B, C, H, N, D) pool")
-    if values is not None:
-        _check_codes(values, "values")
-        if values.codes.shape != keys.codes.shape or values.codes.dtype != keys.codes.dtype:
-            raise ValueError("values must be a pool of the keys' shape and code type")
-    if k_norm_weight.shape != (channels, dim):
-        raise ValueError("k_norm_weight must be (C, D)")
-    if rope_by_slot:
-        if cos.shape != (keys.codes.shape[3], dim) or sin.shape != cos.shape or sin.dtype != cos.dtype:
-            raise ValueError("with rope_by_slot, cos and sin must be (N, D) tables of one dtype")
-    elif cos.shape != (batch, tokens, dim) or sin.shape != cos.shape or sin.dtype != cos.dtype:
-        raise ValueError("cos and sin must be (B, T, D) of one dtype")
-    _check_slots(slots, batch)
-    if slots.shape[-1] != tokens:
-        raise ValueError("slots must be (T,) or (B, T)")
-    _on_gpu("write_pool_quantized", key)
-    torch.ops.white_matter.kv_quant_store(
-        key, value, k_norm_weight, cos, sin, slots, keys.codes, keys.scales, None if values is None else values.codes,
-        None if values is None else values.scales, rope_by_slot, float(eps),
+    # (shapes, types, devices and strides are checked by the operator)
+    key_codes, key_scales = _parts(keys, "keys")
+    value_codes, value_scales = _parts(values, "values")
+    _store(
+        key, value, k_norm_weight, cos, sin, slots, key_codes, key_scales, value_codes, value_scales, rope_by_slot, eps,
     )
 
 
 def quantize_pool(rows: torch.Tensor, dtype: torch.dtype = torch.float8_e4m3fn) -> QuantizedPool:
     """A new quantised pool of the given rows (B, C, H, N, D) float32 or
     bfloat16: what `write_pool` wrote during a prefill, for a decode over it."""
-    _forward_only("quantize_pool", rows)
     if dtype not in _CODE_DTYPES:
         raise ValueError(f"a quantised pool holds float8_e4m3fn or int8 codes, not {dtype}")
-    if rows.ndim != 5 or rows.shape[-1] not in _HEAD_DIMS:
-        raise ValueError("rows must be (B, C, H, N, D) with head_dim 64, 96 or 128")
-    _dtype(rows, "rows")
-    _on_gpu("quantize_pool", rows)
     codes = torch.empty(rows.shape, device=rows.device, dtype=dtype)
     scales = torch.empty(rows.shape[:-1], device=rows.device, dtype=torch.float32)
-    torch.ops.white_matter.kv_quant_store(None, rows, None, None, None, None, None, None, codes, scales, False, 0.0)
+    _store(None, rows, None, None, None, None, None, None, codes, scales, False, 0.0)
     return QuantizedPool(codes, scales)
 
 
@@ -277,23 +234,16 @@ def read_pool(pool: QuantizedPool, slots: torch.Tensor | None = None) -> torch.T
     """bf16(codes * scales) of a quantised pool (B, C, H, N, D): every slot, or
     slots (T,) or (B, T) (one list per batch row) in their order, as a new
     (B, C, H, T, D) tensor. A slot outside [0, N) reads as zeros."""
-    _check_codes(pool, "pool")
-    if slots is not None:
-        _check_slots(slots, pool.codes.shape[0])
-    _on_gpu("read_pool", pool.codes)
-    return torch.ops.white_matter.kv_quant_read(pool.codes, pool.scales, slots)
+    return _read(*_parts(pool, "pool"), slots)
 
 
-def _forward_only(name: str, *tensors: torch.Tensor | None) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name} is forward-only")
-
-
-def _on_gpu(name: str, t: torch.Tensor) -> None:
-    if not t.is_cuda:
-        raise RuntimeError(f"{name} runs on the HIP kernels: it takes GPU tensors")
-
-
+# kv_quant_store(key, value, weight, cos, sin, slots, key_codes, key_scales,
+#     value_codes, value_scales, rope_by_slot, eps) -> (): either side None;
+#     without weight, cos and sin the rows are quantised as they are; without
+#     slots token t goes to slot t
+_store = torch.ops.white_matter.kv_quant_store.default
+# kv_quant_read(codes, scales, slots) -> (B, C, H, T, D) bf16
+_read = torch.ops.white_matter.kv_quant_read.default
 torch.library.register_fake("white_matter::kv_quant_store", lambda *args: None)
 
 

@@ -21,6 +21,13 @@ from . import _native, portable
 _native.load_ops()
 
 
+# token_scores(logits, tokens, top_k, ignore_index) -> (log_probs, entropy,
+#     top_log_probs, top_indices, lse), differentiable in logits; and its
+#     argument checks alone, for any device
+_token_scores = torch.ops.white_matter.token_scores.default
+_token_scores_check = torch.ops.white_matter.token_scores_check.default
+
+
 class TokenLogProbs(NamedTuple):
     """Results of token_log_probs, one row of logits each, float32."""
 
@@ -34,7 +41,7 @@ class TokenLogProbs(NamedTuple):
 def _(logits, tokens, top_k, ignore_index):
     rows = [logits.new_empty(tokens.shape, dtype=torch.float32) for _ in range(3)]
     top = logits.new_empty((*tokens.shape, top_k), dtype=torch.float32)
-    return rows[0], rows[1], top, tokens.new_empty((*tokens.shape, top_k)), rows[2]
+    return rows[0], rows[1], top, tokens.new_empty((*tokens.shape, top_k), dtype=torch.int64), rows[2]
 
 
 @torch.library.register_fake("white_matter::token_scores_bwd")
@@ -59,17 +66,9 @@ def token_log_probs(
     tokens) have probability 0; a row of nothing else has log probabilities
     -inf, entropy 0 and no gradient. A row with a NaN or +inf has NaN results.
     """
-    if logits.ndim < 1 or logits.dtype not in (torch.float32, torch.bfloat16, torch.float16):
-        raise TypeError(f"logits must be float32, bfloat16 or float16 (..., V), got {logits.dtype}")
-    if tokens.dtype not in (torch.int32, torch.int64) or tokens.shape != logits.shape[:-1]:
-        raise ValueError("tokens must be integer, one per row of logits")
-    if tokens.device != logits.device:
-        raise ValueError("tokens must be on the logits' device")
-    most = min(logits.shape[-1], _native.SCORE_MAX_TOP_K)
-    if not 0 <= top_k <= most or logits.shape[-1] < 1:
-        raise ValueError(f"top_k must be in [0, {most}] for {logits.shape[-1]} logits, got {top_k}")
-    if tokens.dtype != torch.int64:
-        tokens = tokens.long()
-    if not logits.is_cuda:
-        return TokenLogProbs(*portable.token_log_probs_portable(logits, tokens, top_k, ignore_index))
-    return TokenLogProbs(*torch.ops.white_matter.token_scores(logits, tokens, top_k, ignore_index)[:4])
+    # (shapes, types and devices are checked by the operator)
+    if logits.is_cuda:
+        scores = _token_scores(logits, tokens, top_k, ignore_index)
+        return TokenLogProbs(scores[0], scores[1], scores[2], scores[3])
+    _token_scores_check(logits, tokens, top_k)
+    return TokenLogProbs(*portable.token_log_probs_portable(logits, tokens.long(), top_k, ignore_index))

@@ -27,11 +27,18 @@ from typing import Literal
 import torch
 
 from . import _kernels, _native, portable
-from .kv_pool import QuantizedPool, _check_codes
+from .kv_pool import QuantizedPool
 
 _native.load_ops()
 
 _BACKENDS = ("auto", "reference", "hip")
+
+
+# tree_attention(query, key, value, key_scales, value_scales, kv_lengths,
+#     kv_length, tree_mask, key_mask, use_dummy, scale, num_splits) ->
+#     (B, n, H, D) bf16, and its argument checks alone, for any device
+_tree_attention = torch.ops.white_matter.tree_attention.default
+_tree_attention_check = torch.ops.white_matter.tree_attention_check.default
 
 
 @torch.library.register_fake("white_matter::tree_attention")
@@ -111,68 +118,34 @@ def tree_attention(
         raise ValueError(f"unsupported tree attention backend: {backend!r}")
     if type(use_dummy_token) is not bool:
         raise ValueError("use_dummy_token must be boolean")
-    quantised = isinstance(key, QuantizedPool)
-    if quantised != isinstance(value, QuantizedPool):
-        raise ValueError("keys and values must both be tensors or both be quantised pools")
-    if quantised:
-        _check_codes(key, "key", 4)
-        _check_codes(value, "value", 4)
-        if key.codes.dtype != value.codes.dtype:
-            raise ValueError("key and value codes must be of one type")
-        k, v, key_scales, value_scales = key.codes, value.codes, key.scales, value.scales
-    else:
-        k, v, key_scales, value_scales = key, value, None, None
-    if query.ndim != 4 or k.ndim != 4 or k.shape != v.shape:
-        raise ValueError("Q/K/V require (B,H,T,D) tensors with matching K/V")
-    batch, heads, nodes, dim = query.shape
-    if k.shape[0] != batch or k.shape[3] != dim or not k.shape[1] or heads % k.shape[1]:
-        raise ValueError("Q/K/V require matching batch/head_dim and divisible heads")
-    if k.device != query.device or v.device != query.device:
-        raise ValueError("Q/K/V must share a device")
-    if not query.is_floating_point():
-        raise ValueError("queries must be floating point")
-    if torch.is_grad_enabled() and (query.requires_grad or (not quantised and (k.requires_grad or v.requires_grad))):
-        raise RuntimeError("tree_attention is forward-only")
-    lengths = kv_lengths if isinstance(kv_lengths, torch.Tensor) else None
-    if lengths is None:
-        if type(kv_lengths) is not int:
-            raise ValueError("kv_lengths must be an integer or integer (B,)")
-    elif lengths.shape != (batch,) or lengths.dtype not in (torch.int32, torch.int64):
+    k, key_scales = key if isinstance(key, QuantizedPool) else (key, None)
+    v, value_scales = value if isinstance(value, QuantizedPool) else (value, None)
+    lengths, length = (kv_lengths, 0) if isinstance(kv_lengths, torch.Tensor) else (None, kv_lengths)
+    if type(length) is not int:
         raise ValueError("kv_lengths must be an integer or integer (B,)")
-    if tree_mask is not None and (
-        tree_mask.dtype != torch.bool or tree_mask.shape not in ((nodes, nodes), (batch, nodes, nodes)) or tree_mask.device != query.device
-    ):
-        raise ValueError("tree_mask must be boolean (n,n) or (B,n,n) on the query's device")
-    if key_mask is not None and (
-        key_mask.dtype != torch.bool or key_mask.shape != (batch, k.shape[2]) or key_mask.device != query.device
-    ):
-        raise ValueError("key_mask must be boolean (B,N) on the query's device")
-    if use_dummy_token and not k.shape[2]:
-        raise ValueError("dummy-enabled K/V must contain the leading dummy slot")
-    if num_splits < 0:
-        raise ValueError("num_splits must not be negative")
+    dim = query.shape[-1]
     scale = dim**-0.5 if softmax_scale is None else float(softmax_scale)
-    if backend == "auto":
-        backend = "hip" if query.is_cuda else "reference"
-    length = 0 if lengths is not None else kv_lengths
-    if backend == "reference":
+    # (shapes, types, devices and strides are checked by the operator)
+    if backend == "reference" or not query.is_cuda:
+        _tree_attention_check(
+            query, k, v, key_scales, value_scales, lengths, length, tree_mask, key_mask, use_dummy_token, scale, num_splits
+        )
+        if backend == "hip":
+            raise ValueError("the HIP backend requires GPU tensors")
         return portable.tree_attention_portable(
             query, k, v, key_scales, value_scales, length if lengths is None else lengths, tree_mask, use_dummy_token, key_mask,
             scale,
         )
-    if not query.is_cuda:
-        raise ValueError("the HIP backend requires GPU tensors")
     padded = _kernels.kernel_head_dim(dim)
     if padded is None:
         raise RuntimeError(f"the gfx950 attention kernels: this path does not support head_dim {dim} (maximum 128)")
-    if not scale > 0:
-        raise RuntimeError(f"the gfx950 attention kernels: this path does not support softmax_scale {scale}")
-    q = query
-    if padded != dim:  # (quantised pools hold the kernels' head_dims)
-        q, k, v = (_kernels.pad_head_dim(t, padded) for t in (q, k, v))
-    out = torch.ops.white_matter.tree_attention(
-        q, k, v, key_scales, value_scales, lengths, length, tree_mask, key_mask, use_dummy_token, scale, num_splits
-    )
-    if padded != dim:
-        out = out[..., :dim]
+    if padded == dim or key_scales is not None:
+        out = _tree_attention(
+            query, k, v, key_scales, value_scales, lengths, length, tree_mask, key_mask, use_dummy_token, scale, num_splits
+        )
+    else:
+        q, k, v = (_kernels.pad_head_dim(t, padded) for t in (query, k, v))
+        out = _tree_attention(
+            q, k, v, None, None, lengths, length, tree_mask, key_mask, use_dummy_token, scale, num_splits
+        )[..., :dim]
     return out if out.dtype == query.dtype else out.to(query.dtype)
