@@ -68,6 +68,18 @@ struct Logit {
     else if constexpr (DT == WMX_DTYPE_BF16) ((bf16*)row)[j] = (bf16)x;
     else ((_Float16*)row)[j] = (_Float16)x;
   }
+  // This thread's vectors of a chunk, from element j on; all loads in flight at
+  // once where the chunk lies whole in the row.
+  static __device__ __forceinline__ void load_chunk(const void* row, int64_t begin, int64_t j, int64_t vocab, u32x4 (&w)[kScoreLoads]) {
+    if (begin + kChunk <= vocab) {
+      const char* p = (const char*)row + j * kSize;
+#pragma unroll
+      for (int i = 0; i < kScoreLoads; ++i) w[i] = __builtin_nontemporal_load((const u32x4_any*)(p + i * kScoreThreads * 16));
+    } else {
+#pragma unroll
+      for (int i = 0; i < kScoreLoads; ++i) w[i] = load(row, j + (int64_t)i * kScoreThreads * kPer, vocab);
+    }
+  }
   // The vector at element j of a row, -inf past its end.
   static __device__ __forceinline__ u32x4 load(const void* row, int64_t j, int64_t vocab) {
     if (j + kPer <= vocab) {
@@ -141,6 +153,48 @@ __device__ __forceinline__ float token_logit(const wmx_score_args& a, const void
   return token >= 0 && token < a.vocab ? Logit<DT>::one(base, token) : 0.f;
 }
 
+// A chunk's top_k entries in order, by one entry at a time: the largest key
+// below the last one. For chunks in which too many values are equal, or too few
+// are finite, for the bound below; reads the chunk again for each entry (from
+// registers, its keys would take all of them in the common case too).
+template <int DT>
+__device__ __forceinline__ void select_slowly(const void* base, int64_t j0, int64_t vocab, int k, uint64_t* entries, uint64_t* lds) {
+  using L = Logit<DT>;
+  constexpr int P = L::kPer;
+  uint64_t last = ~0ull;
+#pragma unroll 1
+  for (int r = 0; r < k; ++r) {
+    uint64_t top = 0;
+#pragma unroll 1
+    for (int i = 0; i < kScoreLoads; ++i) {
+      float x[P];
+      L::unpack(L::load(base, j0 + (int64_t)i * kScoreThreads * P, vocab), x);
+#pragma unroll
+      for (int e = 0; e < P; ++e) {
+        const int64_t j = j0 + (int64_t)i * kScoreThreads * P + e;
+        const uint64_t key = j < vocab ? entry_key(x[e], j) : 0;
+        if (key < last && key > top) top = key;
+      }
+    }
+    top = block_reduce(top, lds, [](uint64_t p, uint64_t q) { return p > q ? p : q; });
+    if (threadIdx.x == 0) entries[r] = top;  // 0: the chunk has no further entry
+    last = top;
+  }
+}
+
+// Rank of `key` among the first n of `found` (distinct keys), two at a time;
+// found[n] exists and is zero where n is odd.
+__device__ __forceinline__ int rank_of(uint64_t key, const uint64_t* found, int n) {
+  typedef uint64_t u64x2 __attribute__((ext_vector_type(2)));
+  int rank = 0;
+#pragma unroll 4
+  for (int i = 0; i < n; i += 2) {
+    const u64x2 other = *(const u64x2*)(found + i);
+    rank += (other[0] > key) + (other[1] > key);
+  }
+  return rank;
+}
+
 // One chunk of one row. TOP: whether entries are selected.
 template <int DT, bool TOP>
 __global__ __launch_bounds__(kScoreThreads) void score_kernel(const wmx_score_args a, int chunks) {
@@ -154,16 +208,17 @@ __global__ __launch_bounds__(kScoreThreads) void score_kernel(const wmx_score_ar
   const int64_t j0 = (int64_t)chunk * L::kChunk + tid * P;  // this thread's vectors: j0 + i * 256 P
 
   u32x4 w[kScoreLoads];
-#pragma unroll
-  for (int i = 0; i < kScoreLoads; ++i) w[i] = L::load(base, j0 + (int64_t)i * kScoreThreads * P, a.vocab);
+  L::load_chunk(base, (int64_t)chunk * L::kChunk, j0, a.vocab, w);
 
-  float mine = kNegInf;
+  float best[kScoreLoads], mine = kNegInf;  // of each vector, of all
 #pragma unroll
   for (int i = 0; i < kScoreLoads; ++i) {
     float x[P];
     L::unpack(w[i], x);
+    best[i] = x[0];
 #pragma unroll
-    for (int e = 0; e < P; ++e) mine = fmaxf(mine, x[e]);
+    for (int e = 1; e < P; ++e) best[i] = fmaxf(best[i], x[e]);
+    mine = fmaxf(mine, best[i]);
   }
   const float m = block_reduce(mine, red, [](float p, float q) { return fmaxf(p, q); });
   const float ref = m == kNegInf ? 0.f : m;
@@ -184,93 +239,63 @@ __global__ __launch_bounds__(kScoreThreads) void score_kernel(const wmx_score_ar
   s = block_reduce(s, red, add);
   t = block_reduce(t, red, add);
 
-  uint64_t* entries = nullptr;  // this chunk's top_k, sorted
   if constexpr (TOP) {
-    __shared__ uint64_t found[kScoreCandidates];
-    __shared__ uint32_t quads[64];
+    __shared__ __attribute__((aligned(16))) uint64_t found[kScoreCandidates];
+    __shared__ __attribute__((aligned(16))) float quads[64];
     __shared__ uint64_t keys[kScoreThreads / 64];
+    __shared__ float bound_lds;
     __shared__ int count;
     const int k = a.top_k;
-    ScorePart* parts = (ScorePart*)a.workspace;
-    entries = (uint64_t*)(parts + a.rows * chunks) + (row * chunks + chunk) * (int64_t)k;
+    uint64_t* entries = (uint64_t*)((ScorePart*)a.workspace + a.rows * chunks) + (row * chunks + chunk) * (int64_t)k;
     // A bound that at least k entries reach: the k-th largest of the maxima of
-    // 64 groups of four threads (k <= 32). Entries above it come from fewer
-    // than k groups.
-    uint32_t best = 0;
-#pragma unroll
-    for (int i = 0; i < kScoreLoads; ++i) {
-      float x[P];
-      L::unpack(w[i], x);
-#pragma unroll
-      for (int e = 0; e < P; ++e) {
-        const int64_t j = j0 + (int64_t)i * kScoreThreads * P + e;
-        const uint32_t o = j < a.vocab ? order_of(x[e]) : 0u;
-        best = best > o ? best : o;
-      }
-    }
-#pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
-      const uint32_t other = __shfl_xor(best, o);
-      best = best > other ? best : other;
-    }
+    // 64 groups of four threads (k <= 32); the entries above it come from
+    // fewer than k groups.
+    float quad = fmaxf(mine, __shfl_xor(mine, 1));
+    quad = fmaxf(quad, __shfl_xor(quad, 2));
     if (tid == 0) count = 0;
-    if ((tid & 3) == 0) quads[tid >> 2] = best;
+    if ((tid & 3) == 0) quads[tid >> 2] = quad;
     __syncthreads();
     if (tid < 64) {
-      const uint32_t q = quads[tid];
+      const float q = quads[tid];
       int above = 0;
-      for (int i = 0; i < 64; ++i) above += quads[i] > q || (quads[i] == q && i < tid);
-      if (above == k - 1) keys[0] = q;
+#pragma unroll
+      for (int i = 0; i < 64; i += 4) {
+        const f32x4 o = *(const f32x4*)(quads + i);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) above += (o[u] > q) + (o[u] == q && i + u < tid);
+      }
+      if (above == k - 1) bound_lds = q;
     }
     __syncthreads();
-    const uint32_t bound = (uint32_t)keys[0];
-    __syncthreads();
-    if (bound != 0) {  // (0: fewer than k groups hold entries)
+    const float bound = bound_lds;
+    // (a chunk with a NaN or +inf has the sum NaN)
+    const bool plain = bound > kNegInf && s == s;
+    if (plain && mine >= bound) {
 #pragma unroll
       for (int i = 0; i < kScoreLoads; ++i) {
+        if (best[i] < bound) continue;
         float x[P];
         L::unpack(w[i], x);
 #pragma unroll
         for (int e = 0; e < P; ++e) {
-          const int64_t j = j0 + (int64_t)i * kScoreThreads * P + e;
-          if (j < a.vocab && order_of(x[e]) >= bound) {
-            const int at = atomicAdd(&count, 1);
-            if (at < kScoreCandidates) found[at] = entry_key(x[e], j);
-          }
+          if (x[e] < bound) continue;  // (past the row's end: -inf)
+          const int at = atomicAdd(&count, 1);
+          if (at < kScoreCandidates) found[at] = entry_key(x[e], j0 + (int64_t)i * kScoreThreads * P + e);
         }
       }
     }
     __syncthreads();
     const int n = count;
-    if (bound != 0 && n <= kScoreCandidates) {
-      // distinct keys: an entry's rank is the number of larger ones
+    if (plain && n <= kScoreCandidates) {
+      if (tid == 0 && (n & 1)) found[n] = 0;  // (n odd is below the capacity, which is even)
+      __syncthreads();
       for (int c = tid; c < n; c += kScoreThreads) {
         const uint64_t key = found[c];
-        int rank = 0;
-        for (int i = 0; i < n; ++i) rank += found[i] > key;
+        const int rank = rank_of(key, found, n);
         if (rank < k) entries[rank] = key;
       }
     } else {
-      // many equal values (or a chunk of few): one entry at a time, the largest
-      // key below the last
-      uint64_t last = ~0ull;
-      for (int r = 0; r < k; ++r) {
-        uint64_t top = 0;
-#pragma unroll
-        for (int i = 0; i < kScoreLoads; ++i) {
-          float x[P];
-          L::unpack(w[i], x);
-#pragma unroll
-          for (int e = 0; e < P; ++e) {
-            const int64_t j = j0 + (int64_t)i * kScoreThreads * P + e;
-            const uint64_t key = j < a.vocab ? entry_key(x[e], j) : 0;
-            if (key < last && key > top) top = key;
-          }
-        }
-        top = block_reduce(top, keys, [](uint64_t p, uint64_t q) { return p > q ? p : q; });
-        if (tid == 0) entries[r] = top;  // 0: the chunk has no further entry
-        last = top;
-      }
+      select_slowly<DT>(base, j0, a.vocab, k, entries, keys);
     }
   }
   if (tid == 0) {
@@ -280,13 +305,39 @@ __global__ __launch_bounds__(kScoreThreads) void score_kernel(const wmx_score_ar
 }
 
 // One wave per row: the chunks' statistics and sorted entries merged.
+constexpr int kMergeEntries = 1024;  // entries of a row that are merged in LDS
 template <int DT>
 __global__ __launch_bounds__(64) void score_merge_kernel(const wmx_score_args a, int chunks) {
+  __shared__ __attribute__((aligned(16))) uint64_t found[kMergeEntries + 2];
+  __shared__ int count;
   const int64_t row = blockIdx.x;
-  const int lane = threadIdx.x;
+  const int lane = threadIdx.x, k = a.top_k;
+  const int64_t n = (int64_t)chunks * k;
   const ScorePart* parts = (const ScorePart*)a.workspace + row * chunks;
+  const uint64_t* entries = (const uint64_t*)((const ScorePart*)a.workspace + a.rows * chunks) + row * n;
+  const void* base = (const char*)a.logits + row * a.row_stride * Logit<DT>::kSize;
+  const float x_token = token_logit<DT>(a, base, row);
+  const auto largest = [](auto p, auto q) { return p > q ? p : q; };
   float m = kNegInf;
   for (int c = lane; c < chunks; c += 64) m = fmaxf(m, parts[c].m);
+  // A bound that at least k entries reach, and its entries: each chunk has
+  // ceil(k / chunks) of them at or above the least of the chunks' such entries.
+  const bool in_lds = k > 0 && n <= kMergeEntries;
+  if (in_lds) {
+    const int each = (k + chunks - 1) / chunks;
+    uint64_t least = ~0ull;
+    for (int c = lane; c < chunks; c += 64) {
+      const uint64_t e = entries[(int64_t)c * k + each - 1];
+      least = e < least ? e : least;
+    }
+    least = ~wave_reduce(~least, largest);
+    if (lane == 0) count = 0;
+    __syncthreads();
+    for (int i = lane; i < n; i += 64) {
+      const uint64_t e = entries[i];
+      if (e >= least && e != 0) found[atomicAdd(&count, 1)] = e;
+    }
+  }
   m = wave_reduce(m, [](float p, float q) { return fmaxf(p, q); });
   const float ref = m == kNegInf ? 0.f : m;
   float s = 0.f, t = 0.f;
@@ -299,26 +350,37 @@ __global__ __launch_bounds__(64) void score_merge_kernel(const wmx_score_args a,
   const auto add = [](float p, float q) { return p + q; };
   s = wave_reduce(s, add);
   t = wave_reduce(t, add);
-  const void* base = (const char*)a.logits + row * a.row_stride * Logit<DT>::kSize;
-  if (lane == 0) finish_row(a, row, m, s, t, token_logit<DT>(a, base, row));
-  const int k = a.top_k;
+  if (lane == 0) finish_row(a, row, m, s, t, x_token);
   if (k == 0) return;
-  const uint64_t* entries = (const uint64_t*)((const ScorePart*)a.workspace + a.rows * chunks) + row * chunks * (int64_t)k;
   const float log_s = logf(s);
   const bool empty = m == kNegInf && s == 0.f;
-  // the next of all chunks' entries k times: the largest key below the last
+  const auto put = [&](int rank, uint64_t key) {
+    a.top_indices[row * k + rank] = entry_index(key);
+    a.top_log_probs[row * k + rank] = empty ? kNegInf : (value_of((uint32_t)(key >> 32)) - ref) - log_s;
+  };
+  if (in_lds) {
+    __syncthreads();
+    const int found_n = count;
+    if (lane == 0) found[found_n] = 0;
+    __syncthreads();
+    for (int c = lane; c < found_n; c += 64) {
+      const uint64_t key = found[c];
+      const int rank = rank_of(key, found, found_n);
+      if (rank < k) put(rank, key);
+    }
+    return;
+  }
+  // rows of very many chunks: the next of all entries k times, the largest key
+  // below the last
   uint64_t last = ~0ull;
   for (int r = 0; r < k; ++r) {
     uint64_t top = 0;
-    for (int i = lane; i < chunks * k; i += 64) {
+    for (int64_t i = lane; i < n; i += 64) {
       const uint64_t key = entries[i];
       if (key < last && key > top) top = key;
     }
-    top = wave_reduce(top, [](uint64_t p, uint64_t q) { return p > q ? p : q; });
-    if (lane == 0) {
-      a.top_indices[row * k + r] = entry_index(top);
-      a.top_log_probs[row * k + r] = empty ? kNegInf : (value_of((uint32_t)(top >> 32)) - ref) - log_s;
-    }
+    top = wave_reduce(top, largest);
+    if (lane == 0) put(r, top);
     last = top;
   }
 }
@@ -337,8 +399,7 @@ __global__ __launch_bounds__(kScoreThreads) void score_bwd_kernel(const wmx_scor
   const int64_t begin = (int64_t)chunk * L::kChunk, j0 = begin + tid * P;
 
   u32x4 w[kScoreLoads];
-#pragma unroll
-  for (int i = 0; i < kScoreLoads; ++i) w[i] = L::load(base, j0 + (int64_t)i * kScoreThreads * P, a.vocab);
+  L::load_chunk(base, begin, j0, a.vocab, w);
 
   const float lse = a.lse[row], entropy = a.entropy[row];
   const int64_t token = a.tokens[row];
