@@ -806,9 +806,10 @@ typedef struct wmx_kv_read_args {
  * visible slot produce zeros.
  * q (B, Hq, n, D) and o in bf16, strides [batch, head, node]; k/v pool strides
  * [batch, head, slot] in elements of the format, scales [batch, head] with unit
- * stride along the slots (WMX_POOL_BF16: none). Rows of q and of a bf16 pool
- * are 16-byte aligned, rows of codes 8-byte aligned (16 for head_dim 64 and
- * 128), o 4-byte; a slot stride is below 2^25 bytes.
+ * stride along the slots (WMX_POOL_BF16: none). Rows of q, o and of a bf16
+ * pool are 16-byte aligned, rows of codes 8-byte aligned (16 for head_dim 64
+ * and 128); a slot stride is below 2^25 bytes. With num_splits 0 the work is
+ * dealt out by the lengths (up to 256 batch rows).
  */
 typedef struct wmx_tree_args {
   const void* q;
@@ -839,7 +840,7 @@ typedef struct wmx_tree_args {
   int32_t capacity;          /* pool slots N */
   int32_t head_dim;          /* 64, 96 or 128 */
   int32_t use_dummy;
-  int32_t num_splits;        /* key splits; 0 chooses */
+  int32_t num_splits;        /* key ranges of every row and KV head; 0 chooses */
   float softmax_scale;       /* positive */
 } wmx_tree_args;
 
@@ -1034,7 +1035,6 @@ int wmx_plan_fill(const wmx_plan_args* args, void* stream);
  * reference, whose pools are bf16 and whose decode takes one token. */
 int wmx_kv_quant_store(const wmx_kv_quant_args* args, void* stream);
 int wmx_kv_quant_read(const wmx_kv_read_args* args, void* stream);
-int32_t wmx_tree_num_splits(const wmx_tree_args* args);
 int64_t wmx_tree_workspace_size(const wmx_tree_args* args);
 int wmx_tree_attn(const wmx_tree_args* args, void* stream);
 

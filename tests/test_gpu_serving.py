@@ -357,6 +357,50 @@ def test_tree_attention_padded_head_dim():
     _assert_tree(out, _tree_reference(query, key, value, [50, 50], tree, False, None, 80**-0.5))
 
 
+@pytest.mark.parametrize("kind", ["bf16", "e4m3", "int8"])
+@pytest.mark.parametrize(("batch", "heads", "kv_heads", "nodes"), [(1, 2, 1, 1), (6, 4, 2, 1), (6, 4, 2, 19), (70, 2, 1, 3), (256, 1, 1, 1), (257, 1, 1, 1)])
+@torch.no_grad()
+def test_tree_attention_deals_ragged_batches(kind, batch, heads, kv_heads, nodes):
+    """Pools long enough for work dealt out by the lengths: most rows short, some
+    empty, few long, with and without a key mask that leaves ranges empty; the
+    same launch captured, and replayed after the lengths have changed."""
+    print(f"dealt {kind} B={batch} H={heads}/{kv_heads} n={nodes}", flush=True)
+    gen, capacity, dim = _gen(batch + nodes), 1700, 64
+    key, value, k, v = _pool_pair(gen, (batch, kv_heads, capacity, dim), kind)
+    query = _randn(gen, batch, heads, nodes, dim)
+    tree = _random_tree(gen, batch, nodes)
+    mask = torch.rand(batch, capacity, generator=gen) < 0.5
+    mask[:, 300:900] = False
+    mask = mask.to(DEV)
+    first = torch.randint(0, 140, (batch,), generator=gen)
+    first[::3] = 0
+    first[batch // 2 :: 7] = capacity - nodes
+    second = first.flip(0).contiguous()
+    second[-1] = 1300
+    lengths = first.to(DEV)
+
+    def run(key_mask):
+        return tree_attention(query, key, value, kv_lengths=lengths, tree_mask=tree, key_mask=key_mask, softmax_scale=0.2)
+
+    for key_mask in (None, mask):
+        _assert_tree(run(key_mask), _tree_reference(query, k, v, first, tree, False, key_mask, 0.2))
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        run(None)
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(None)
+    for at in (second, first, second):
+        lengths.copy_(at)
+        graph.replay()
+        eager = run(None)
+        torch.cuda.synchronize()
+        _assert_tree(out, _tree_reference(query, k, v, at, tree, False, None, 0.2))
+        assert torch.equal(out, eager)
+
+
 @pytest.mark.parametrize("kind", ["bf16", "int8"])
 @torch.no_grad()
 def test_tree_attention_long_context(kind):

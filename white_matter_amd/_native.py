@@ -438,7 +438,6 @@ EXPORTS = (
     "wmx_plan_fill",
     "wmx_kv_quant_store",
     "wmx_kv_quant_read",
-    "wmx_tree_num_splits",
     "wmx_tree_workspace_size",
     "wmx_tree_attn",
     "wmx_score_workspace_size",

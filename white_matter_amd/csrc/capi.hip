@@ -730,7 +730,6 @@ static int check_tree(const wmx_tree_args* a) {
   return WMX_OK;
 }
 
-int32_t wmx_tree_num_splits(const wmx_tree_args* a) { return check_tree(a) ? 0 : wmx::tree_num_splits(*a); }
 int64_t wmx_tree_workspace_size(const wmx_tree_args* a) { return check_tree(a) ? 0 : wmx::tree_workspace_size(*a); }
 
 int wmx_tree_attn(const wmx_tree_args* a, void* stream) {
@@ -740,8 +739,7 @@ int wmx_tree_attn(const wmx_tree_args* a, void* stream) {
   if (!a->q || !a->o || (a->capacity > 0 && (!a->k || !a->v || (codes && (!a->k_scales || !a->v_scales)))))
     return fail(WMX_E_INVALID, "tree attention pointer is NULL");
   if (!aligned16(a->q) || !strides_vec8(a->q_stride, 3)) return fail(WMX_E_INVALID, "q must be 16-byte aligned rows");
-  if (((uintptr_t)a->o & 3u) || a->o_stride[0] % 2 || a->o_stride[1] % 2 || a->o_stride[2] % 2)
-    return fail(WMX_E_INVALID, "o must be 4-byte aligned rows");
+  if (!aligned16(a->o) || !strides_vec8(a->o_stride, 3)) return fail(WMX_E_INVALID, "o must be 16-byte aligned rows");
   // rows of codes are read 16 bytes at a time, at head_dim 96 8 bytes
   const int64_t unit = !codes ? 8 : a->head_dim == 96 ? 8 : 16;
   const uintptr_t low = (codes && a->head_dim == 96) ? 7u : 15u;

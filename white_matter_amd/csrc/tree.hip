@@ -21,30 +21,20 @@
 // of one per element. Codes are converted exactly: K's to bf16 like the
 // queries; V's to fp16, in which the weights keep 11 bits (bf16 pools: 8).
 #include <climits>
-
 #include "wmx_kernels.h"
 
 namespace wmx {
 
-constexpr int kTreeWaves = 4;
-constexpr int kTreeTile = 32;                      // slots per wave and step
-constexpr int kTreeStep = kTreeWaves * kTreeTile;  // slots per workgroup and step
 // The running maximum follows a larger score only once it is past it by this
 // many powers of two: weights up to 2^8 cost no precision, and most steps
 // rescale nothing.
 constexpr float kLazyMax = 8.f;
-// V scales are multiplied by a power of two that keeps them at most 64, so that
-// weights times scales stay below 2^14 in fp16 (largest 65,504).
+// V scales times 2^lv stay at most 64, so that weights times scales stay below
+// 2^14 in fp16 (largest 65,504).
 constexpr float kScaleRoom = 64.f;
 
-__device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a), as_bf16x8(b), c, 0, 0, 0);
-}
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-__device__ __forceinline__ f32x4 mfma16_half(const u32x4& a, const u32x4& b, const f32x4& c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
 
 // Two codes (the low or high half of a dword) as a bf16 or fp16 pair, exactly.
 template <int FMT, bool HIGH>
@@ -77,6 +67,82 @@ __device__ __forceinline__ tree_rsrc tree_buffer(const char* base, int bytes) {
                                            0x00020000);
 }
 constexpr int kReadOnce = 2;  // cache policy: nontemporal
+
+// A value as if it changed here: what is derived from it (the lane masks of its
+// bits, a pair of scalar registers each) is formed at its use and not kept.
+__device__ __forceinline__ void fresh(uint32_t& x) { __asm__ volatile("" : "+v"(x)); }
+
+struct TreeRange {
+  int base;   // committed slots (every node sees them)
+  int total;  // committed and drafted slots, within the pool
+};
+
+__device__ __forceinline__ TreeRange tree_range(const wmx_tree_args& a, int b) {
+  int64_t len = a.kv_lengths ? a.kv_lengths[b] : a.kv_length_scalar;
+  len = len < 0 ? 0 : len;
+  const int64_t cap = a.capacity;
+  int64_t base = len > cap ? cap : len + a.use_dummy;
+  base = base > cap ? cap : base;
+  const int64_t total = a.tree_mask ? min(base + a.nodes, cap) : base;
+  return TreeRange{__builtin_amdgcn_readfirstlane((int)base), __builtin_amdgcn_readfirstlane((int)total)};
+}
+
+// The weights of a query row are x = exp2(t - ref), t its scaled scores in powers
+// of two and ref = m - lv: m a score near the largest so far, 2^lv a factor that
+// keeps weights times V scales within fp16 (0 for bf16 pools). Sums and outputs
+// hold x and its products; `limit` is the t - ref from which ref moves: lv +
+// kLazyMax, or -inf until the row has seen a slot.
+struct TreeRow {
+  float ref, limit, l;
+
+  __device__ __forceinline__ void start(float lv) {
+    ref = -lv;
+    limit = kNegInf;
+    l = 0.f;
+  }
+  // For lanes of rows with a score past their limit (top: the row's largest t -
+  // ref): how far ref moves, and the factor that sums and outputs take.
+  __device__ __forceinline__ float move(float top, float lv, float& factor) {
+    const bool seen = limit != kNegInf;
+    float up = top - lv;
+    up = seen ? fmaxf(up, 0.f) : top == kNegInf ? 0.f : up;
+    factor = seen ? __builtin_amdgcn_exp2f(-up) : 1.f;  // (nothing to scale before the first slot)
+    ref += up;
+    l *= factor;
+    limit = seen || top > kNegInf ? lv + kLazyMax : kNegInf;
+    return up;
+  }
+  // Another lv, `by` larger; `factor` = 2^by.
+  __device__ __forceinline__ void rescale(float by, float factor) {
+    ref -= by;
+    limit += by;
+    l *= factor;
+  }
+  // The maximum that goes with l / 2^lv.
+  __device__ __forceinline__ float max_score(float lv) const { return limit == kNegInf ? kNegInf : ref + lv; }
+};
+
+// The lv that takes the largest V scale `most` of a tile (over the wave) into
+// [32, 64) for the weight 1, and the one to begin with: any but the smallest
+// scales replace it, and sums of 2^lv stay finite.
+__device__ __forceinline__ float scale_lv(float most) {
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o));
+  return (float)min(132 - (int)(__float_as_uint(most) >> 23), 100);
+}
+constexpr float kScaleStart = 100.f;
+
+constexpr int kTreeWaves = 4;
+constexpr int kTreeTile = 32;                      // slots per wave and step
+constexpr int kTreeStep = kTreeWaves * kTreeTile;  // slots per workgroup and step
+
+__device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a), as_bf16x8(b), c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma16_half(const u32x4& a, const u32x4& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
 
 // How a wave reads 32 slots of K and V.
 template <int FMT, int D>
@@ -178,23 +244,12 @@ struct TreeTile {
   static constexpr uint32_t kOdd = FMT == WMX_POOL_BF16 ? 0x7f80u : 0x7c00u;
 };
 
-// A value as if it changed here: what is derived from it (the lane masks of its
-// bits, a pair of scalar registers each) is formed at its use and not kept.
-__device__ __forceinline__ void fresh(uint32_t& x) { __asm__ volatile("" : "+v"(x)); }
-
-struct TreeRange {
-  int base;   // committed slots (every node sees them)
-  int total;  // committed and drafted slots, within the pool
-};
-
-__device__ __forceinline__ TreeRange tree_range(const wmx_tree_args& a, int b) {
+// Steps of a batch row, per KV head (one at least: its outputs are written).
+__device__ __forceinline__ int tree_steps(const wmx_tree_args& a, int b) {
   int64_t len = a.kv_lengths ? a.kv_lengths[b] : a.kv_length_scalar;
-  len = len < 0 ? 0 : len;
-  const int64_t cap = a.capacity;
-  int64_t base = len > cap ? cap : len + a.use_dummy;
-  base = base > cap ? cap : base;
-  const int64_t total = a.tree_mask ? min(base + a.nodes, cap) : base;
-  return TreeRange{__builtin_amdgcn_readfirstlane((int)base), __builtin_amdgcn_readfirstlane((int)total)};
+  len = len < 0 ? 0 : len > a.capacity ? a.capacity : len + a.use_dummy;
+  const int64_t total = min(a.tree_mask ? len + a.nodes : len, (int64_t)a.capacity);
+  return max(1, (int)((total + kTreeStep - 1) / kTreeStep));
 }
 
 // x of lanes l ^ 16 and l ^ 32 joined with this lane's, the same in all four
@@ -214,9 +269,9 @@ struct TreeWave {
   static constexpr int KS = Tile::KS, W = Tile::W;
 
   u32x4 qf[MB][KS];  // queries, the B operand
-  float m[MB], l[MB];
+  TreeRow row[MB];
   f32x4 acc[MB][W];
-  float vref;        // V scales are multiplied by it (a power of two)
+  float lv, vref;    // (vref = 2^lv)
   Tile tile;
   float ks[8], vs[8];
   int koff[2], voff[8];
@@ -319,13 +374,14 @@ struct TreeWave {
           for (int mb = 0; mb < MB; ++mb) s[mb][u] = mfma16(kf, qf[mb][st], s[mb][u]);
         }
       }
+      // scores over the reference: the weights are exp2 of them
       float kq[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) kq[e] = FMT == WMX_POOL_BF16 ? scale : scale * ks[e];
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) sc[mb][e] = s[mb][e >> 2][e & 3] * kq[e];
+        for (int e = 0; e < 8; ++e) sc[mb][e] = fmaf(s[mb][e >> 2][e & 3], kq[e], -row[mb].ref);
       }
     }
     const int next = j0 + kTreeStep;
@@ -343,22 +399,20 @@ struct TreeWave {
     if constexpr (FMT != WMX_POOL_BF16) {
       float most = 0.f;  // (NaN stays out of it, and an infinity)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) most = fmaxf(most, vs[e] < kPosInf ? vs[e] : 0.f);
+      for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(vs[e]) < kPosInf ? fabsf(vs[e]) : 0.f);
       if (__any(most * vref > kScaleRoom)) {
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) most = fmaxf(most, __shfl_xor(most, o));
-        const int up = 132 - (int)(__float_as_uint(most) >> 23);  // most * 2^up in [32, 64)
-        const float ref = __uint_as_float((uint32_t)(127 + min(up, 120)) << 23);
-        const float f = ref / vref;
+        const float to = scale_lv(most), f = __builtin_amdgcn_exp2f(to - lv);
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb) {
+          row[mb].rescale(to - lv, f);
 #pragma unroll
           for (int c = 0; c < W; ++c) acc[mb][c] *= f;
-        }
-        vref = ref;
-      }
 #pragma unroll
-      for (int e = 0; e < 8; ++e) vs[e] *= vref;
+          for (int e = 0; e < 8; ++e) sc[mb][e] += to - lv;
+        }
+        lv = to;
+        vref = __builtin_amdgcn_exp2f(lv);
+      }
     }
 
     u32x4 p[MB];  // weights (times V scales), the B operand
@@ -367,21 +421,20 @@ struct TreeWave {
       float top = fmaxf(sc[mb][0], sc[mb][1]);
 #pragma unroll
       for (int e = 2; e < 8; ++e) top = fmaxf(top, sc[mb][e]);
-      if (__any(top > m[mb] + kLazyMax)) {
-        const float mn = fmaxf(m[mb], max_quarters(top));
-        const float f = mn == kNegInf ? 0.f : __builtin_amdgcn_exp2f(m[mb] - mn);
-        l[mb] *= f;
+      if (__any(top > row[mb].limit)) {
+        float f;
+        const float up = row[mb].move(max_quarters(top), lv, f);
 #pragma unroll
         for (int c = 0; c < W; ++c) acc[mb][c] *= f;
-        m[mb] = mn;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sc[mb][e] -= up;
       }
-      const float ref = m[mb] == kNegInf ? 0.f : m[mb];
       float x[8];
       if constexpr (EDGE) fresh(seen[mb]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        x[e] = __builtin_amdgcn_exp2f(sc[mb][e] - ref);
-        l[mb] += x[e];
+        x[e] = __builtin_amdgcn_exp2f(sc[mb][e]);
+        row[mb].l += x[e];
         if constexpr (FMT != WMX_POOL_BF16) {
           x[e] *= vs[e];
           if constexpr (EDGE) x[e] = (seen[mb] >> e) & 1u ? x[e] : 0.f;  // a masked row's scale may be NaN
@@ -443,31 +496,124 @@ struct TreeWave {
   }
 };
 
+// Which key range a workgroup takes. The slots of every (batch row, KV head), the
+// drafted ones included, are counted in steps of kTreeStep. With nsplit 0 the
+// workgroups are dealt out by these counts: all steps over `ranges` give a share,
+// a (row, head) of n steps gets ceil(n / share) workgroups, and these split its
+// steps evenly; a row of one writes the outputs itself. Rows of any lengths then
+// load the card alike, whatever the pool's capacity. With nsplit > 0 every (row,
+// head) has that many ranges of `share` steps.
+struct TreeLaunch {
+  int tiles, ranges, nsplit, share;
+};
+// Pools of up to so many steps (1,280 slots) are not split: the second launch and
+// the partials cost more than idle CUs do (600 slots: 8 rows of one node 12 us,
+// 16 us dealt; 32 rows of 64 nodes 30 and 36. 1,280 slots: 10.0 and 13.5 us for a
+// row, 8 rows of 16 nodes 19.2 and 17.2. 2,500 slots: 16.5 and 14.2 us for a row,
+// 8 rows 25 and 17).
+constexpr int kOneRange = 10;
+constexpr int kPlanRows = 256;  // most batch rows whose workgroups are dealt out
+// How the steps are dealt, by the query rows of a workgroup: 16 rows stream the
+// slots, and four workgroups a CU, of at least four steps, are best (e4m3, D 128,
+// 8 KV heads, up to 8,192 slots: 32 rows 68 us, 71 with two a CU, 75 with twelve;
+// 8 rows 27 us, 32 with workgroups of two steps). With 32 rows the arithmetic sets
+// the pace: one a CU, of any length (64 nodes over 16 x 8,192 slots 119 us, 124
+// with two a CU; 4 x 1,500 slots 14 us, 17 with four steps at least).
+__host__ __device__ constexpr int tree_dealt(int rows) { return rows == 16 ? 1024 : 256; }
+__host__ __device__ constexpr int tree_min_share(int rows) { return rows == 16 ? 4 : 1; }
+// At the workspace's start, for the merge: the ranges before each row (per KV head), and all.
+constexpr int kPlanInts = 512;
+struct TreePartials {
+  float *ml, *o;
+};
+__host__ __device__ inline int64_t tree_partial_rows(const TreeLaunch& t, int rows) {
+  return (int64_t)t.ranges * t.tiles * rows;
+}
+__device__ __forceinline__ TreePartials tree_partials(const wmx_tree_args& a, const TreeLaunch& t, int rows) {
+  float* o = (float*)a.workspace + kPlanInts;
+  return TreePartials{o + tree_partial_rows(t, rows) * a.head_dim, o};
+}
+
 template <int FMT, int D, int MB>
-__global__ __launch_bounds__(64 * kTreeWaves, (MB == 1 && TreeTile<FMT, D>::kRow < 256) ? 3 : 2) void tree_kernel(const wmx_tree_args a, int units, int tiles,
-                                                                          int nsplit, int chunk) {
+__global__ __launch_bounds__(64 * kTreeWaves, (MB == 1 && TreeTile<FMT, D>::kRow < 256) ? 3 : 2) void tree_kernel(
+    const wmx_tree_args a, const TreeLaunch t) {
   using Tile = TreeTile<FMT, D>;
   constexpr int KS = Tile::KS, W = Tile::W, ROWS = 16 * MB;
   constexpr int LDR = 4 * W + 4;  // LDS row of one merge round: four quarters x W, padded against bank conflicts
   __shared__ __attribute__((aligned(16))) float lds_o[kTreeWaves][ROWS][LDR];
   __shared__ float lds_m[kTreeWaves][ROWS], lds_l[kTreeWaves][ROWS], lds_max[ROWS], lds_sum[ROWS];
-  __shared__ int lds_odd;
+  __shared__ int lds_odd, lds_wave[kTreeWaves], lds_all[kTreeWaves], lds_first[4];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
   const int li = lane & 15, q = lane >> 4;
-  // blocks 8 apart share an XCD: the row tiles of one (range, row, KV head)
-  // are placed so, and read its slots through one L2
-  const int slab = blockIdx.x / (8 * tiles), in_slab = blockIdx.x - slab * 8 * tiles;
-  const int unit = slab * 8 + (in_slab & 7), tile_row = in_slab >> 3;
-  if (unit >= units) return;
-  const int pairs = a.batch * a.kv_heads;
-  const int split = unit / pairs, pair = unit - split * pairs;
-  const int b = pair / a.kv_heads, hk = pair - b * a.kv_heads;
+  // blocks 8 apart share an XCD: the row tiles of one range are placed so, and
+  // read its slots through one L2
+  const int slab = blockIdx.x / (8 * t.tiles), in_slab = blockIdx.x - slab * 8 * t.tiles;
+  const int index = slab * 8 + (in_slab & 7), tile_row = in_slab >> 3;  // of the range, of the row tile
+  if (index >= t.ranges) return;
   const int group = a.q_heads / a.kv_heads;
   const int rows = a.nodes * group, row0 = tile_row * ROWS;
 
+  // ---- the range: steps [s0, s1) of (b, hk) ----
+  int b, hk, s0, s1, parts;
+  if (t.nsplit > 0) {
+    const int unit = index / t.nsplit;
+    b = unit / a.kv_heads;
+    hk = unit - b * a.kv_heads;
+    s0 = (index - unit * t.nsplit) * t.share;
+    s1 = s0 + t.share;
+    parts = t.nsplit;
+  } else {
+    const int steps = tid < a.batch ? tree_steps(a, tid) : 0;
+    int sum = steps;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
+    if (lane == 0) lds_wave[wave] = sum;
+    __syncthreads();
+    int all = 0;
+#pragma unroll
+    for (int i = 0; i < kTreeWaves; ++i) all += lds_wave[i];
+    const int share = max(tree_min_share(ROWS), (all * a.kv_heads + t.share - 1) / t.share);
+    const int n = (steps + share - 1) / share;
+    int before = n;  // inclusive scan over the workgroup
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int up = __shfl_up(before, o);
+      before += lane >= o ? up : 0;
+    }
+    if (lane == 63) lds_all[wave] = before;
+    __syncthreads();
+    int ranges = 0;
+#pragma unroll
+    for (int i = 0; i < kTreeWaves; ++i) {
+      before += i < wave ? lds_all[i] : 0;
+      ranges += lds_all[i];
+    }
+    before -= n;
+    if (index == 0 && tile_row == 0) {
+      int* plan = (int*)a.workspace;
+      if (tid < a.batch) plan[tid] = before;
+      if (tid == 0) plan[a.batch] = ranges;
+    }
+    if (index >= ranges * a.kv_heads) return;
+    if (index >= before * a.kv_heads && index < (before + n) * a.kv_heads) {
+      lds_first[0] = tid;
+      lds_first[1] = index - before * a.kv_heads;
+      lds_first[2] = n;
+      lds_first[3] = steps;
+    }
+    __syncthreads();
+    b = __builtin_amdgcn_readfirstlane(lds_first[0]);
+    const int at = __builtin_amdgcn_readfirstlane(lds_first[1]), total = __builtin_amdgcn_readfirstlane(lds_first[3]);
+    parts = __builtin_amdgcn_readfirstlane(lds_first[2]);
+    hk = at / parts;
+    const int part = at - hk * parts, each = total / parts, more = total - each * parts;
+    s0 = part * each + min(part, more);
+    s1 = s0 + each + (part < more);
+  }
   const TreeRange range = tree_range(a, b);
-  const int begin = split * chunk, end = min(begin + chunk, range.total);
+  const bool complete = parts == 1;
+  const int begin = min(s0 * kTreeStep, range.total), end = min(s1 * kTreeStep, range.total);
   const uint8_t* kmask = a.key_mask ? a.key_mask + (int64_t)b * a.key_mask_stride : nullptr;
   const uint8_t* tmask = a.tree_mask ? a.tree_mask + (int64_t)b * a.tree_mask_stride[0] : nullptr;
   const char* vbase = (const char*)a.v + ((int64_t)b * a.v_stride[0] + (int64_t)hk * a.v_stride[1]) * Tile::kElem;
@@ -475,12 +621,12 @@ __global__ __launch_bounds__(64 * kTreeWaves, (MB == 1 && TreeTile<FMT, D>::kRow
   if (tid == 0) lds_odd = 0;
 
   TreeWave<FMT, D, MB> w;
-  w.vref = 0x1p120f;
+  w.lv = FMT == WMX_POOL_BF16 ? 0.f : kScaleStart;
+  w.vref = __builtin_amdgcn_exp2f(w.lv);
   w.odd = false;
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) {
-    w.m[mb] = kNegInf;
-    w.l[mb] = 0.f;
+    w.row[mb].start(w.lv);
 #pragma unroll
     for (int c = 0; c < W; ++c) w.acc[mb][c] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
@@ -529,19 +675,18 @@ __global__ __launch_bounds__(64 * kTreeWaves, (MB == 1 && TreeTile<FMT, D>::kRow
 
   // the workgroup's waves merged: maxima and sums, then the outputs in four
   // rounds (round r: block rows 4 q + r, W consecutive d per lane)
+  float m[MB];
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) {
-    w.l[mb] = sum_quarters(w.l[mb]);
+    m[mb] = w.row[mb].max_score(w.lv);
+    const float l = sum_quarters(w.row[mb].l) * (1.f / w.vref);
     if (q == 0) {
-      lds_m[wave][16 * mb + li] = w.m[mb];
-      lds_l[wave][16 * mb + li] = w.l[mb];
+      lds_m[wave][16 * mb + li] = m[mb];
+      lds_l[wave][16 * mb + li] = l;
     }
   }
   __syncthreads();
   if (w.odd) lds_odd = 1;
-  float* ws_o = (float*)a.workspace;
-  float* ws_ml = ws_o + (int64_t)a.batch * a.q_heads * a.nodes * nsplit * D;
-  const int64_t prow0 = ((int64_t)pair * rows + row0) * nsplit + split;  // partial of row row0; rows are nsplit apart
   // per row: the maximum over the waves, and what the outputs are divided by
   if (tid < ROWS) {
     float mx = lds_m[0][tid], sum = 0.f;
@@ -557,100 +702,117 @@ __global__ __launch_bounds__(64 * kTreeWaves, (MB == 1 && TreeTile<FMT, D>::kRow
     lds_sum[tid] = sum;
   }
   __syncthreads();
-  if (nsplit > 1 && tid < min(ROWS, rows - row0)) {
-    float* out = ws_ml + (prow0 + (int64_t)tid * nsplit) * 2;
+  const TreePartials part = tree_partials(a, t, ROWS);
+  const int64_t prow0 = ((int64_t)index * t.tiles + tile_row) * ROWS;
+  if (!complete && tid < ROWS) {
+    float* out = part.ml + (prow0 + tid) * 2;
     out[0] = lds_max[tid];
     out[1] = lds_sum[tid];
   }
-  if (nsplit > 1 && begin >= end) return;  // (the workgroup agrees) its sum is zero: the merge skips it
-  float factor[MB];  // this wave's share of its rows
-#pragma unroll
-  for (int mb = 0; mb < MB; ++mb) {
-    const int row = 16 * mb + li;
-    const float f = w.m[mb] == kNegInf ? 1.f : __builtin_amdgcn_exp2f(w.m[mb] - lds_max[row]);
-    const float sum = nsplit > 1 ? 1.f : lds_sum[row];
-    factor[mb] = sum == 0.f ? 0.f : f / sum;
-    if constexpr (FMT != WMX_POOL_BF16) factor[mb] *= 1.f / w.vref;
-  }
-  constexpr int PAIRS = ROWS * 4 * W / 2;  // output pairs of a round
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    __syncthreads();
+  // (an empty range's sums are zero: the merge skips its outputs)
+  if (complete || begin < end) {
+    float factor[MB];  // this wave's share of its rows
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) {
-#pragma unroll
-      for (int c = 0; c < W; c += 2) {
-        float* dst = &lds_o[wave][16 * mb + li][W * q + c];
-        dst[0] = w.acc[mb][c][r] * factor[mb];
-        dst[1] = w.acc[mb][c + 1][r] * factor[mb];
-      }
+      const int row = 16 * mb + li;
+      const float f = m[mb] == kNegInf ? 1.f : __builtin_amdgcn_exp2f(m[mb] - lds_max[row]);
+      const float sum = complete ? lds_sum[row] : 1.f;
+      factor[mb] = sum == 0.f ? 0.f : f / sum * (1.f / w.vref);
     }
-    __syncthreads();
-    for (int i = tid; i < PAIRS; i += 64 * kTreeWaves) {
-      const int row = i / (2 * W), x = i - row * 2 * W;
-      const int qq = x / (W / 2), c = 2 * (x - qq * (W / 2));
-      if (row0 + row >= rows) continue;
-      float o0 = 0.f, o1 = 0.f;
+    constexpr int PAIRS = ROWS * 4 * W / 2;  // output pairs of a round
 #pragma unroll
-      for (int i4 = 0; i4 < kTreeWaves; ++i4) {
-        o0 += lds_o[i4][row][W * qq + c];
-        o1 += lds_o[i4][row][W * qq + c + 1];
-      }
-      const int d = Tile::v_dim(4 * qq + r, c);  // (c even: d and d + 1)
-      const int n = (row0 + row) / group, h = hk * group + (row0 + row - n * group);
-      if (FMT != WMX_POOL_INT8 && lds_odd) {
-        // drafted values that are not finite, for the queries that see them:
-        // any positive weight leaves them as they are
-        for (int j = max(begin, range.base); j < end; ++j) {
-          if (!tmask[(int64_t)n * a.tree_mask_stride[1] + (j - range.base)] || (kmask && !kmask[j])) continue;
-          const char* at = vbase + j * vsb + d * Tile::kElem;
-          float v0, v1;
-          if constexpr (FMT == WMX_POOL_BF16) {
-            v0 = bf16_lo(*(const uint32_t*)at);
-            v1 = bf16_hi(*(const uint32_t*)at);
-          } else {  // (only NaN)
-            const uint32_t u = *(const uint16_t*)at;
-            v0 = (u & 0x7fu) == 0x7fu ? __builtin_nanf("") : 0.f;
-            v1 = (u & 0x7f00u) == 0x7f00u ? __builtin_nanf("") : 0.f;
-          }
-          o0 += __builtin_isfinite(v0) ? 0.f : v0;
-          o1 += __builtin_isfinite(v1) ? 0.f : v1;
+    for (int r = 0; r < 4; ++r) {
+      __syncthreads();
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) {
+#pragma unroll
+        for (int c = 0; c < W; c += 2) {
+          float* dst = &lds_o[wave][16 * mb + li][W * q + c];
+          dst[0] = w.acc[mb][c][r] * factor[mb];
+          dst[1] = w.acc[mb][c + 1][r] * factor[mb];
         }
       }
-      if (nsplit > 1) {
-        float* out = ws_o + (prow0 + (int64_t)row * nsplit) * D + d;
-        out[0] = o0;
-        out[1] = o1;
-      } else {
-        bf16* out = (bf16*)a.o + (int64_t)b * a.o_stride[0] + (int64_t)h * a.o_stride[1] + (int64_t)n * a.o_stride[2] + d;
-        *(uint32_t*)out = pack_bf16x2(o0, o1);
+      __syncthreads();
+      for (int i = tid; i < PAIRS; i += 64 * kTreeWaves) {
+        const int row = i / (2 * W), x = i - row * 2 * W;
+        const int qq = x / (W / 2), c = 2 * (x - qq * (W / 2));
+        if (row0 + row >= rows) continue;
+        float o0 = 0.f, o1 = 0.f;
+#pragma unroll
+        for (int i4 = 0; i4 < kTreeWaves; ++i4) {
+          o0 += lds_o[i4][row][W * qq + c];
+          o1 += lds_o[i4][row][W * qq + c + 1];
+        }
+        const int d = Tile::v_dim(4 * qq + r, c);  // (c even: d and d + 1)
+        const int n = (row0 + row) / group, h = hk * group + (row0 + row - n * group);
+        if (FMT != WMX_POOL_INT8 && lds_odd) {
+          // drafted values that are not finite, for the queries that see them:
+          // any positive weight leaves them as they are
+          for (int j = max(begin, range.base); j < end; ++j) {
+            if (!tmask[(int64_t)n * a.tree_mask_stride[1] + (j - range.base)] || (kmask && !kmask[j])) continue;
+            const char* at = vbase + j * vsb + d * Tile::kElem;
+            float v0, v1;
+            if constexpr (FMT == WMX_POOL_BF16) {
+              v0 = bf16_lo(*(const uint32_t*)at);
+              v1 = bf16_hi(*(const uint32_t*)at);
+            } else {  // (only NaN)
+              const uint32_t u = *(const uint16_t*)at;
+              v0 = (u & 0x7fu) == 0x7fu ? __builtin_nanf("") : 0.f;
+              v1 = (u & 0x7f00u) == 0x7f00u ? __builtin_nanf("") : 0.f;
+            }
+            o0 += __builtin_isfinite(v0) ? 0.f : v0;
+            o1 += __builtin_isfinite(v1) ? 0.f : v1;
+          }
+        }
+        if (complete) {
+          bf16* out = (bf16*)a.o + (int64_t)b * a.o_stride[0] + (int64_t)h * a.o_stride[1] + (int64_t)n * a.o_stride[2] + d;
+          *(uint32_t*)out = pack_bf16x2(o0, o1);
+        } else {
+          float* out = part.o + (prow0 + row) * D + d;
+          out[0] = o0;
+          out[1] = o1;
+        }
       }
     }
   }
 }
 
 // Merge of a row's ranges: one thread per four consecutive d, eight ranges'
-// loads in flight.
-__global__ __launch_bounds__(256) void tree_merge_kernel(const wmx_tree_args a, int nsplit, int64_t threads) {
+// loads in flight. `rows_wg`: query rows of a range's workgroup.
+__global__ __launch_bounds__(256) void tree_merge_kernel(const wmx_tree_args a, const TreeLaunch t, int rows_wg, int64_t threads) {
   const int64_t gid = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (gid >= threads) return;
   const int D = a.head_dim, per = D / 4, group = a.q_heads / a.kv_heads, rows = a.nodes * group;
   const int64_t row = gid / per;
   const int d = 4 * (int)(gid - row * per);
-  const float* ws_o = (const float*)a.workspace;
+  const int64_t pair = row / rows;
+  const int in_pair = (int)(row - pair * rows), n = in_pair / group;
+  const int b = (int)(pair / a.kv_heads), hk = (int)(pair - (int64_t)b * a.kv_heads), h = hk * group + in_pair - n * group;
+  const int tile = in_pair / rows_wg;
+  int64_t first;
+  int count;
+  if (t.nsplit > 0) {
+    first = pair * t.nsplit;
+    count = t.nsplit;
+  } else {
+    const int* plan = (const int*)a.workspace;
+    count = plan[b + 1] - plan[b];
+    if (count == 1) return;  // (written by its workgroup)
+    first = plan[b] * a.kv_heads + hk * count;
+  }
   typedef float f32x2 __attribute__((ext_vector_type(2)));
-  const f32x2* ws_ml = (const f32x2*)(ws_o + (int64_t)a.batch * a.q_heads * a.nodes * nsplit * D) + row * nsplit;
-  ws_o += row * nsplit * D + d;
+  const TreePartials part = tree_partials(a, t, rows_wg);
+  const int64_t part0 = (first * t.tiles + tile) * rows_wg + (in_pair - tile * rows_wg), part_step = (int64_t)t.tiles * rows_wg;
   float mx = kNegInf, sum = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int s0 = 0; s0 < nsplit; s0 += 8) {
+  for (int s0 = 0; s0 < count; s0 += 8) {
     f32x2 ml[8];
-    f32x4 part[8];
+    f32x4 po[8];
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
-      const int s = min(s0 + u, nsplit - 1);
-      ml[u] = ws_ml[s];
-      part[u] = *(const f32x4*)(ws_o + (int64_t)s * D);  // an empty range wrote none: not used
+      const int64_t r = part0 + min(s0 + u, count - 1) * part_step;
+      ml[u] = *(const f32x2*)(part.ml + r * 2);
+      po[u] = *(const f32x4*)(part.o + r * D + d);  // an empty range wrote none: not used
     }
     float top = mx;
 #pragma unroll
@@ -661,58 +823,55 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const wmx_tree_args a, 
     mx = top;
 #pragma unroll
     for (int u = 0; u < 8; ++u) {
-      if (s0 + u >= nsplit || ml[u][1] == 0.f) continue;
+      if (s0 + u >= count || ml[u][1] == 0.f) continue;
       const float w = ml[u][0] == kNegInf ? 1.f : __builtin_amdgcn_exp2f(ml[u][0] - top);
       sum += ml[u][1] * w;
-      o += part[u] * w;
+      o += po[u] * w;
     }
   }
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
-  const int64_t pair = row / rows;
-  const int in_pair = (int)(row - pair * rows), n = in_pair / group;
-  const int b = (int)(pair / a.kv_heads), hk = (int)(pair - (int64_t)b * a.kv_heads), h = hk * group + in_pair - n * group;
   bf16* out = (bf16*)a.o + (int64_t)b * a.o_stride[0] + (int64_t)h * a.o_stride[1] + (int64_t)n * a.o_stride[2] + d;
   const u32x2 w = {pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv)};
-  typedef u32x2 u32x2_4 __attribute__((aligned(4)));
-  *(u32x2_4*)out = w;
+  *(u32x2*)out = w;
 }
 
-// Query rows per workgroup in 16s. Two 16s use 240 registers, two waves a SIMD;
-// three and four share the conversions further but leave one wave a SIMD
+// Query rows per workgroup: 16 or 32. Two 16s use 240 registers, two waves a
+// SIMD; three and four share the conversions further but leave one wave a SIMD
 // (measured: 64 nodes x 2 heads over 16 x 8,192 slots 128 us with two, 167 with
 // four, 194 with three).
-static int tree_blocks(const wmx_tree_args& a) { return (int64_t)a.nodes * (a.q_heads / a.kv_heads) <= 16 ? 1 : 2; }
-static int64_t tree_workgroups(const wmx_tree_args& a) {  // per key range
-  const int64_t rows = (int64_t)a.nodes * (a.q_heads / a.kv_heads), per = 16 * tree_blocks(a);
-  return (rows + per - 1) / per * a.batch * a.kv_heads;
-}
+static int tree_rows(const wmx_tree_args& a) { return (int64_t)a.nodes * (a.q_heads / a.kv_heads) <= 16 ? 16 : 32; }
 
-int tree_num_splits(const wmx_tree_args& a) {
-  if (a.num_splits > 0) return a.num_splits;
-  const int64_t wgs = tree_workgroups(a);
-  if (wgs <= 0) return 1;
-  int64_t splits = (4 * 256 + wgs - 1) / wgs;
-  const int64_t most = ((int64_t)a.capacity + 255) / 256;
-  if (splits > most) splits = most;
-  return splits < 1 ? 1 : (int)splits;
+static TreeLaunch tree_plan(const wmx_tree_args& a) {
+  const int64_t rows = (int64_t)a.nodes * (a.q_heads / a.kv_heads), per = tree_rows(a);
+  const int64_t tiles = (rows + per - 1) / per, pairs = (int64_t)a.batch * a.kv_heads;
+  const int64_t most = max(1, (a.capacity + kTreeStep - 1) / kTreeStep);  // steps of a (row, head)
+  TreeLaunch t{};
+  t.tiles = (int)tiles;
+  if (a.num_splits > 0) {
+    t.nsplit = a.num_splits;
+  } else if (most <= kOneRange || a.batch > kPlanRows || pairs * most > (1 << 30)) {
+    t.nsplit = 1;
+  } else {
+    const int64_t least = tree_min_share((int)per);
+    t.share = (int)max((int64_t)1, tree_dealt((int)per) / tiles);  // workgroups to deal the steps over
+    t.ranges = (int)min(pairs + t.share, pairs * ((most + least - 1) / least));
+    return t;
+  }
+  t.share = (int)((most + t.nsplit - 1) / t.nsplit);
+  t.ranges = (int)min((int64_t)INT32_MAX, pairs * t.nsplit);
+  return t;
 }
 
 int64_t tree_workspace_size(const wmx_tree_args& a) {
-  const int64_t s = tree_num_splits(a);
-  return s == 1 ? 0 : (int64_t)a.batch * a.q_heads * a.nodes * s * (a.head_dim + 2) * (int64_t)sizeof(float);
+  const TreeLaunch t = tree_plan(a);
+  return t.nsplit == 1 ? 0 : 4 * (kPlanInts + tree_partial_rows(t, tree_rows(a)) * (a.head_dim + 2));
 }
-
-struct TreeLaunch {
-  int units, tiles, nsplit, chunk;
-};
 
 template <int FMT, int D>
 static void launch_tree_d(const wmx_tree_args& a, unsigned blocks, const TreeLaunch& t, hipStream_t stream) {
   const dim3 grid(blocks), block(64 * kTreeWaves);
-  if (tree_blocks(a) == 1)
-    hipLaunchKernelGGL((tree_kernel<FMT, D, 1>), grid, block, 0, stream, a, t.units, t.tiles, t.nsplit, t.chunk);
-  else
-    hipLaunchKernelGGL((tree_kernel<FMT, D, 2>), grid, block, 0, stream, a, t.units, t.tiles, t.nsplit, t.chunk);
+  if (tree_rows(a) == 16) hipLaunchKernelGGL((tree_kernel<FMT, D, 1>), grid, block, 0, stream, a, t);
+  else hipLaunchKernelGGL((tree_kernel<FMT, D, 2>), grid, block, 0, stream, a, t);
 }
 
 template <int FMT>
@@ -726,22 +885,18 @@ static int launch_tree_f(const wmx_tree_args& a, unsigned blocks, const TreeLaun
 }
 
 int launch_tree(const wmx_tree_args& a, hipStream_t stream) {
-  const int nsplit = tree_num_splits(a);
-  const int64_t pairs = (int64_t)a.batch * a.kv_heads, units = nsplit * pairs, tiles = tree_workgroups(a) / pairs;
-  const int64_t blocks = (units + 7) / 8 * 8 * tiles;
+  const TreeLaunch t = tree_plan(a);
+  const int64_t blocks = ((int64_t)t.ranges + 7) / 8 * 8 * t.tiles;
   const int64_t merged = (int64_t)a.batch * a.q_heads * a.nodes * (a.head_dim / 4);
-  if (blocks > INT32_MAX || (merged + 255) / 256 > INT32_MAX) return WMX_E_UNSUPPORTED;
-  int64_t chunk = ((int64_t)a.capacity + nsplit - 1) / nsplit;
-  chunk = (chunk + kTreeStep - 1) / kTreeStep * kTreeStep;
-  if (chunk < kTreeStep) chunk = kTreeStep;
-  if (chunk * nsplit > INT32_MAX) return WMX_E_UNSUPPORTED;  // (ranges begin within 31 bits)
-  const TreeLaunch t{(int)units, (int)tiles, nsplit, (int)chunk};
+  if (blocks > INT32_MAX || (merged + 255) / 256 > INT32_MAX || (int64_t)a.batch * a.kv_heads * max(1, t.nsplit) > INT32_MAX ||
+      (int64_t)t.share * max(1, t.nsplit) * kTreeStep > INT32_MAX)
+    return WMX_E_UNSUPPORTED;  // (ranges are counted, and begin, within 31 bits)
   int rc;
   if (a.format == WMX_POOL_BF16) rc = launch_tree_f<WMX_POOL_BF16>(a, (unsigned)blocks, t, stream);
   else if (a.format == WMX_POOL_E4M3) rc = launch_tree_f<WMX_POOL_E4M3>(a, (unsigned)blocks, t, stream);
   else rc = launch_tree_f<WMX_POOL_INT8>(a, (unsigned)blocks, t, stream);
-  if (rc != WMX_OK || nsplit == 1) return rc;
-  hipLaunchKernelGGL(tree_merge_kernel, dim3((unsigned)((merged + 255) / 256)), dim3(256), 0, stream, a, nsplit, merged);
+  if (rc != WMX_OK || t.nsplit == 1) return rc;
+  hipLaunchKernelGGL(tree_merge_kernel, dim3((unsigned)((merged + 255) / 256)), dim3(256), 0, stream, a, t, tree_rows(a), merged);
   return WMX_OK;
 }
 

@@ -85,7 +85,6 @@ int launch_plan_count(const wmx_plan_args& a, hipStream_t stream);
 int launch_plan_fill(const wmx_plan_args& a, hipStream_t stream);
 int launch_kv_quant(const wmx_kv_quant_args& a, hipStream_t stream);
 int launch_kv_read(const wmx_kv_read_args& a, hipStream_t stream);
-int tree_num_splits(const wmx_tree_args& a);
 int64_t tree_workspace_size(const wmx_tree_args& a);
 int launch_tree(const wmx_tree_args& a, hipStream_t stream);
 int64_t score_workspace_size(const wmx_score_args& a);
