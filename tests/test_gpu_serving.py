@@ -30,6 +30,8 @@ import math
 import pytest
 import torch
 
+from tests.test_gpu_cyclic_pass import _check, _rel_l2, _setup
+from tests.test_serving import TreeOracle
 from white_matter_amd import (
     kv_pool,
     strict_causal_attention,
@@ -37,6 +39,7 @@ from white_matter_amd import (
     tree_attention,
     tree_mask_from_parents,
 )
+from white_matter_amd.cyclic_pass import GreedyDecoder, forward_cyclic, score_drafts
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -697,3 +700,126 @@ def test_compiled_calls():
         eager, compiled = step(query), torch.compile(step, fullgraph=True, backend="aot_eager")(query)
     for a, b in zip((*eager[0], eager[1]), (*compiled[0], compiled[1])):
         assert torch.equal(a, b)
+
+
+# ------------------------------------------------------- drafted decoding ----
+def _pool_oracle(dtype):
+    """The oracle's kernel set over pools of values: stored rows are rounded to
+    the grid of a quantised pool's codes (dtype None: left as they are)."""
+
+    class Rounded(TreeOracle):
+        @staticmethod
+        def store(key, value, weight, cos, sin, keys, values, slots, *, eps):
+            TreeOracle.store(key, value, weight, cos, sin, keys, values, slots, eps=eps)
+            for pool in (keys, values) if dtype else ():
+                rows = pool[..., slots, :].double()
+                scale = rows.abs().amax(-1, keepdim=True) / TOP[dtype]
+                x = rows / torch.where(scale > 0, scale, 1.0)
+                x = x.round() if dtype == INT8 else x.float().to(dtype).double()
+                pool[..., slots, :] = (x * scale).to(pool.dtype)
+
+    return Rounded
+
+
+def _check_stored(hip, ref, exact, dtype, what):
+    """`_check` for pool rows. Where two runs' rows lie on two sides of the
+    middle between codes they are stored one step apart, whose largest size is
+    32 of a row's 448 (e4m3, top binade) or 1 of its 127: a row's largest
+    magnitude times that, past the bf16 bar, is the most they differ by."""
+    if dtype is None:
+        return _check(hip, ref, exact, what)
+    r_hip, m_hip, scale = _rel_l2(hip, exact)
+    r_ref, _, _ = _rel_l2(ref, exact)
+    print(f"{what}: rel_l2 hip {r_hip:.3e} bf16-oracle {r_ref:.3e}, max_abs hip {m_hip:.3e}", flush=True)
+    assert r_hip <= 1.5 * r_ref + 1e-6, f"{what}: HIP rel_l2 {r_hip:.3e} vs bf16 oracle run {r_ref:.3e}"
+    assert m_hip <= 1e-2 * max(1.0, scale) + scale * (1 / 127 if dtype == INT8 else 32 / 448), f"{what}: max_abs {m_hip:.3e}"
+
+
+@pytest.mark.parametrize("dtype", [None, E4M3, INT8])
+@torch.no_grad()
+def test_prefill_decode_and_drafts_run_together(dtype):
+    """A prefill's pool quantised, decoded from (captured and eager), and a tree
+    of drafts run behind it and scored. Against the same weights in float32 over
+    the oracle, the kernels' error is at most 1.5 times that of the bf16 model
+    over the oracle, both over rows rounded to the same grid."""
+    model, exact, ids, docs = _setup()
+    steps, parents = 3, [-1, 0, 0, 1, -1, 4, 3, 2, 2]
+    nodes, used = len(parents), ids.shape[1] + 1
+    capacity = used + steps + nodes
+    hidden, keys, values, positions = forward_cyclic(model, ids, docs, capacity=capacity)
+    if dtype is None:
+        pools, rows = (keys, values), (keys, values)
+    else:
+        pools = tuple(kv_pool.quantize_pool(t, dtype) for t in (keys, values))
+        rows = tuple(_values(p) for p in pools)
+
+    def copy(pool):
+        return pool.clone() if dtype is None else kv_pool.QuantizedPool(*(t.clone() for t in pool))
+
+    def read(pool):
+        return kv_pool.read_pool(pool) if dtype else pool
+
+    oracle = _pool_oracle(dtype)
+    h = hidden.float()
+    hip = GreedyDecoder.after_prefill(model, h, *(copy(p) for p in pools), positions, docs)
+    eager = GreedyDecoder.after_prefill(model, h, *(copy(p) for p in pools), positions, docs, capture=False)
+    ref = GreedyDecoder.after_prefill(model, h, *(r.bfloat16() for r in rows), positions, docs, kernels=oracle, capture=False)
+    full = GreedyDecoder.after_prefill(exact, h, *(r.float() for r in rows), positions, docs, kernels=oracle, capture=False)
+    for step in range(steps):
+        for other in (eager, ref, full):
+            other.token.copy_(hip.token)
+        for decoder in (hip, eager, ref, full):
+            decoder()
+        torch.cuda.synchronize()
+        for name in ("keys", "values"):
+            got, same, want, best = (getattr(d, name) for d in (hip, eager, ref, full))
+            got, same = read(got), read(same)
+            at = used + step
+            assert torch.equal(got, same), "graph replay and eager launches must store the same token"
+            _check_stored(got[..., at, :], want[..., at, :], best[..., at, :], dtype, f"{dtype} step {step} {name}")
+
+    drafts = torch.randint(0, 96, (2, nodes), generator=_gen(3)).to(DEV)
+    context = h[:, -1:]
+    results = []
+    for m, d, kernels in ((model, hip, None), (model, ref, oracle), (exact, full, oracle)):
+        more = {} if kernels is None else dict(kernels=kernels)
+        out, scores = score_drafts(
+            m, drafts, parents, context, d.keys, d.values, used + steps, d.position, d.key_mask, top_k=4, **more,
+        )
+        results.append((out, scores.log_probs, scores.top_log_probs, *(read(p) if kernels is None else p for p in (d.keys, d.values))))
+    torch.cuda.synchronize()
+    names = ("outputs", "log probabilities", "alternatives", "keys", "values")
+    for name, got, want, best in zip(names, *results):
+        if name in ("keys", "values"):
+            got, want, best = (t[..., used + steps :, :] for t in (got, want, best))
+            _check_stored(got, want, best, dtype, f"{dtype} drafts' {name}")
+        else:
+            _check(got, want, best, f"{dtype} drafts' {name}")
+    # committed rows are left as they were
+    for pool, start in zip((hip.keys, hip.values), (eager.keys, eager.values)):
+        for a, b in zip((pool,) if dtype is None else pool, (start,) if dtype is None else start):
+            slots = 3 if dtype is None or a.ndim == 5 else -1
+            assert torch.equal(a.narrow(slots, 0, used + steps).float(), b.narrow(slots, 0, used + steps).float())
+
+
+@torch.no_grad()
+def test_a_drafted_chain_matches_decoding():
+    """The kernels' own decoding of a chain, one token at a time, and the chain
+    as one tree: the pool rows agree to a bf16 model's noise (2^-6 relative in
+    the L2 norm, over 4 bf16 roundings a layer and 3 layers), the scores too."""
+    model, _, ids, docs = _setup()
+    nodes, used = 4, ids.shape[1] + 1
+    hidden, *bf16, positions = forward_cyclic(model, ids, docs, capacity=used + nodes)
+    pools = [kv_pool.quantize_pool(t) for t in bf16]
+    decoder = GreedyDecoder.after_prefill(model, hidden, *(kv_pool.QuantizedPool(*(t.clone() for t in p)) for p in pools), positions, docs)
+    keep, tokens = decoder.key_mask.clone(), []
+    for _ in range(nodes):
+        tokens.append(decoder.token.clone())
+        decoder()
+    drafts = torch.cat(tokens, 1)
+    _, scores = score_drafts(model, drafts, [-1, 0, 1, 2], hidden[:, -1:], *pools, used, positions[:, -1:] + 1, keep, top_k=1)
+    for pool, alone in zip(pools, (decoder.keys, decoder.values)):
+        got, want = (_values(p)[..., used:, :] for p in (pool, alone))
+        assert float((got - want).norm() / want.norm()) < 2**-6
+    # greedy drafts are the top alternative of the rows above them, up to that noise
+    assert (scores.log_probs - scores.top_log_probs[..., 0] >= -0.02).all()

@@ -8,7 +8,9 @@ import math
 import pytest
 import torch
 
+from tests.test_cyclic_pass import OracleKernels, _model
 from white_matter_amd import _native, kv_pool, token_log_probs, tree_attention, tree_mask_from_parents
+from white_matter_amd.cyclic_pass import GreedyDecoder, forward_cyclic, score_drafts
 
 F64 = torch.float64
 
@@ -228,3 +230,66 @@ def test_c_entry_points_refuse_before_launching():
         entry = getattr(lib, name)
         entry.argtypes, entry.restype = [ctypes.c_void_p], ctypes.c_int64
         assert entry(None) == 0 and entry(ctypes.create_string_buffer(1024)) == 0
+
+
+# ---------------------------------------------------------- drafted decoding ----
+class TreeOracle(OracleKernels):
+    @staticmethod
+    def tree(q, k, v, *, lengths, tree_mask, use_dummy_token, key_mask):
+        return tree_attention(
+            q.cpu(), k.cpu(), v.cpu(), kv_lengths=lengths.cpu(), tree_mask=tree_mask.cpu(), use_dummy_token=use_dummy_token,
+            key_mask=None if key_mask is None else key_mask.cpu(), backend="reference",
+        ).to(q.device, q.dtype)
+
+
+@pytest.mark.parametrize("dummy", [True, False])
+@pytest.mark.parametrize("documents", [True, False])
+def test_drafted_paths_match_decoding(dummy, documents):
+    """Every node of a drafted tree has the output, the pool rows and the score
+    that decoding its path one token at a time gives, in float64 to the portable
+    path's float32 scores and weights (2^-24 on sums of up to 40 terms each)."""
+    torch.manual_seed(4)
+    length, parents = 12, [-1, 0, 0, 1, -1, 4, 3]
+    nodes, offset = len(parents), int(dummy)
+    model = _model(length, use_dummy_token=dummy)
+    ids = torch.randint(0, 50, (2, length))
+    docs = torch.tensor([[0] * 5 + [1] * 7, [0] * 9 + [1] * 3]) if documents else None
+    capacity = length + offset + nodes + 1
+    hidden, keys, values, positions = forward_cyclic(model, ids, docs, capacity=capacity, kernels=OracleKernels)
+    keep = torch.zeros(2, capacity, dtype=torch.bool)
+    keep[:, offset : length + offset] = True if docs is None else docs == docs[:, -1:]
+    keep[:, 0] |= dummy
+    drafts = torch.randint(0, 50, (2, nodes))
+    drafted = [t.clone() for t in (keys, values)]
+    out, scores = score_drafts(
+        model, drafts, parents, hidden[:, -1:], *drafted, length + offset, positions[:, -1:] + 1, keep, top_k=3, kernels=TreeOracle,
+    )
+    assert out.shape == (2, nodes, 32) and scores.top_indices.shape == (2, nodes, 3)
+    bound = dict(rtol=2e-5, atol=2e-6)
+    for node in range(nodes):
+        path = [node]
+        while parents[path[0]] >= 0:
+            path.insert(0, parents[path[0]])
+        decoder = GreedyDecoder(
+            model, keys.clone(), values.clone(), length + offset, positions[:, -1:] + 1, drafts[:, :1], keep,
+            kernels=OracleKernels, capture=False,
+        )
+        logits = model.logits(hidden[:, -1:])
+        for step, i in enumerate(path):
+            want = torch.log_softmax(logits[:, 0], -1)
+            decoder.token.copy_(drafts[:, i : i + 1])
+            decoder()
+            at = length + offset + step
+            for got, alone in zip(drafted, (decoder.keys, decoder.values)):
+                assert torch.allclose(got[..., length + offset + i, :], alone[..., at, :], **bound)
+            logits = model.logits(out[:, i : i + 1])
+        given = want.gather(1, drafts[:, node : node + 1])[:, 0]
+        assert torch.allclose(scores.log_probs[:, node].double(), given, rtol=0, atol=2e-5)
+        assert torch.allclose(scores.entropy[:, node].double(), -(want.exp() * want).sum(-1), rtol=0, atol=2e-4)
+        assert torch.allclose(scores.top_log_probs[:, node].double(), want.topk(3)[0], rtol=0, atol=2e-5)
+    with pytest.raises(ValueError, match="free slot"):
+        score_drafts(model, drafts, parents, hidden[:, -1:], *drafted, capacity - nodes + 1, positions[:, -1:], kernels=TreeOracle)
+    with pytest.raises(ValueError, match="context"):
+        score_drafts(model, drafts, parents, hidden, *drafted, length + offset, positions[:, -1:], kernels=TreeOracle)
+    none, empty = score_drafts(model, drafts[:, :0], [], hidden[:, -1:], *drafted, length + offset, positions[:, -1:], kernels=TreeOracle)
+    assert none.shape == (2, 0, 32) and empty.log_probs.shape == (2, 0)

@@ -26,7 +26,10 @@ Inference restatement of the reference's feedback block:
   * cached decoding (models/generation.py:38-100 `DecodeGraph`,
     blocks/white_matter.py:165-186 `_run_token_layers`): one token through
     every layer with the split-K decode kernel over the pool, the token's
-    keys and values stored at the next slot, captured in a HIP graph.
+    keys and values stored at the next slot, captured in a HIP graph, over a
+    bf16 pool or a quantised one (`kv_pool.quantize_pool` of the prefill's);
+  * drafted decoding (`score_drafts`, no counterpart in the reference): a tree
+    of drafted tokens run over the pool at once, and scored.
 
 The model is random-initialised (no checkpoints): projections N(0, 0.02),
 norms and gains one, routers at the reference's "cyclic:0.25" prior with zero
@@ -46,6 +49,8 @@ from . import _kernels, _native, kv_pool
 from .cyclic_attention import cyclic_attention
 from .metadata import prepare_feedback_metadata
 from .strict_causal_attention import strict_causal_attention
+from .token_scores import TokenLogProbs, token_log_probs
+from .tree_attention import tree_attention, tree_mask_from_parents
 
 
 # residual_norm, query_norm_rope and silu_mul (csrc/torch_ops.cpp, layer_ops.hip):
@@ -130,7 +135,8 @@ class FeedbackConfig:
 
 class HipKernels:
     """The attention-path operations of the pass and of decoding, on the HIP
-    kernels. q is (B, Hq, T, D); the pool views are (B, Hkv, N, D)."""
+    kernels. q is (B, Hq, T, D); the pool views are (B, Hkv, N, D), where
+    decoding reads and stores also those of a `kv_pool.QuantizedPool`."""
 
     @staticmethod
     def cyclic(q, k, v, *, query_stride, query_offset, strict_past, metadata):
@@ -144,13 +150,24 @@ class HipKernels:
     @staticmethod
     def decode(q, k, v, *, lengths, use_dummy_token, key_mask):
         """One query per row over the pool's committed slots -> (B, 1, Hq, D)."""
+        if isinstance(k, kv_pool.QuantizedPool):
+            return tree_attention(q, k, v, kv_lengths=lengths, use_dummy_token=use_dummy_token, key_mask=key_mask)
         return strict_causal_attention(
             q, k, v, query_start=lengths, kv_lengths=lengths, use_dummy_token=use_dummy_token, key_mask=key_mask
         )
 
     @staticmethod
+    def tree(q, k, v, *, lengths, tree_mask, use_dummy_token, key_mask):
+        """The queries of drafted tokens over the committed slots and their own
+        ancestors' -> (B, T, Hq, D)."""
+        return tree_attention(
+            q, k, v, kv_lengths=lengths, tree_mask=tree_mask, use_dummy_token=use_dummy_token, key_mask=key_mask
+        )
+
+    @staticmethod
     def store(key, value, k_norm_weight, cos, sin, keys, values, slots, *, eps):
-        kv_pool.write_pool(key, value, k_norm_weight, cos, sin, keys, values, slots, eps=eps)
+        write = kv_pool.write_pool_quantized if isinstance(keys, kv_pool.QuantizedPool) else kv_pool.write_pool
+        write(key, value, k_norm_weight, cos, sin, keys, values, slots, eps=eps)
 
     @staticmethod
     def mix(model: "FeedbackModel", stacked):
@@ -395,6 +412,17 @@ class FeedbackModel:
             return torch.ops.white_matter.residual_norm(x, None, None, self.final_norm, c.rms_norm_eps) @ self.embed.t()
         return self._norm(x, self.final_norm) @ self.embed.t()
 
+    def token_scores(self, x: torch.Tensor, tokens: torch.Tensor, *, top_k: int = 0, chunk: int = 512) -> TokenLogProbs:
+        """`token_log_probs` of tokens (...) under the logits of outputs x (...,
+        d), `chunk` rows of logits at a time."""
+        rows, given = x.reshape(-1, x.shape[-1]), tokens.reshape(-1)
+        parts = []
+        for start in range(0, max(len(given), 1), chunk):
+            logits = self.logits(rows[None, start : start + chunk])[0]
+            logits = logits.float() if logits.dtype == torch.float64 else logits
+            parts.append(token_log_probs(logits, given[start : start + chunk], top_k=top_k))
+        return TokenLogProbs(*(torch.cat(p).view(*tokens.shape, *p[0].shape[1:]) for p in zip(*parts)))
+
     def new_pool(self, batch: int, capacity: int) -> tuple[torch.Tensor, torch.Tensor]:
         c = self.config
         shape = (batch, c.num_kv_channels, c.num_kv_heads, capacity, c.head_dim)
@@ -503,7 +531,7 @@ class GreedyDecoder:
     runs through every layer, layer l attending from its query to pool channel
     l % k over the committed slots (the dummy and the row's last document,
     then every decoded token), and its keys and values are written at the next
-    slot. Static buffers, readable and writable between calls: `token` (B, 1)
+    slot. The pool is the prefill's, or a quantised one of its rows. Static buffers, readable and writable between calls: `token` (B, 1)
     the next input token, `position` (B, 1) its position (before the dummy
     shift), `length` (1,) the slots in use (dummy included; the token is
     written there), `key_mask` (B, N) the slots it may read."""
@@ -568,7 +596,7 @@ class GreedyDecoder:
         def attend(index, q):
             ch = index % c.num_kv_channels
             return self.kernels.decode(
-                q, self.keys[:, ch], self.values[:, ch], lengths=lengths, use_dummy_token=c.use_dummy_token,
+                q, self.keys.select(1, ch), self.values.select(1, ch), lengths=lengths, use_dummy_token=c.use_dummy_token,
                 key_mask=self.key_mask,
             )
 
@@ -593,3 +621,74 @@ class GreedyDecoder:
             self.step()
         self.seen += 1
         return self.token
+
+
+@torch.no_grad()
+def score_drafts(
+    model: FeedbackModel,
+    tokens: torch.Tensor,
+    parents,
+    context: torch.Tensor,
+    keys,
+    values,
+    length: int,
+    position: torch.Tensor,
+    key_mask: torch.Tensor | None = None,
+    *,
+    passes: int | None = None,
+    top_k: int = 0,
+    kernels=HipKernels,
+) -> tuple[torch.Tensor, TokenLogProbs]:
+    """A tree of drafted tokens run behind a pool's `length` slots in use (dummy
+    included), and the score of each under its parent's output.
+
+    tokens (B, n) the drafts, parents (n,) or (B, n) the node that each hangs
+    under (an earlier one, or -1 for the context: `tree_mask_from_parents`),
+    context (B, 1, d) the output of the last committed token, position (B, 1)
+    the position behind it, key_mask (B, N) the committed slots that a row may
+    read; keys and values a bf16 or quantised pool with n free slots.
+
+    A token's keys and values are mixed from its outputs in every layer, so a
+    node is right once its parent is: like the cyclic prefill the slots start
+    from the embeddings, and pass p makes depth p final. The default number of
+    passes, the tree's depth, decodes every path of the tree exactly as one
+    token at a time would; with fewer the deeper nodes hold the passes' estimate.
+    Returns the nodes' outputs (B, n, d) and their scores, shapes (B, n): the
+    node's log probability, and the entropy and alternatives in its place. Node i
+    is left in slot length + i."""
+    c = model.config
+    batch, nodes = tokens.shape
+    offset, sources = int(c.use_dummy_token), c.num_sources
+    if not offset <= length <= keys.shape[3] - nodes:
+        raise ValueError("the pool has no free slot for every drafted token")
+    if context.shape != (batch, 1, c.hidden_size):
+        raise ValueError("context must be (B, 1, d)")
+    if nodes == 0:
+        return context[:, :0], model.token_scores(context[:, :0], tokens, top_k=top_k)
+    device = keys.device
+    parents = torch.as_tensor(parents)
+    tree_mask, depths = tree_mask_from_parents(parents, device="cpu")
+    passes = int(depths.max()) + 1 if passes is None else passes
+    tree_mask, depths = tree_mask.to(device), depths.to(device)
+    x = model.embed[tokens].to(model.residual_dtype)
+    rope = model.rope((position.reshape(-1, 1) + depths).expand(batch, nodes) + offset)
+    slots = torch.arange(length, length + nodes, device=device)
+    lengths = torch.full((batch,), length - offset, device=device, dtype=torch.long)
+    if key_mask is not None:
+        key_mask = key_mask.index_fill(1, slots, True)
+
+    def attend(index, q):
+        ch = index % c.num_kv_channels
+        return kernels.tree(
+            q, keys.select(1, ch), values.select(1, ch), lengths=lengths, tree_mask=tree_mask,
+            use_dummy_token=c.use_dummy_token, key_mask=key_mask,
+        )
+
+    write_sources(model, x[:, :, None].expand(-1, -1, sources, -1), keys, values, slots, rope, kernels)
+    hidden = x
+    for _ in range(passes):
+        hidden, stacked = model.layers_stacked(x, attend, rope)
+        write_sources(model, stacked, keys, values, slots, rope, kernels)
+    above = (parents.to(device) + 1).expand(batch, nodes)[..., None].expand(-1, -1, c.hidden_size)
+    before = torch.cat((context.to(hidden.dtype), hidden), dim=1).gather(1, above)
+    return hidden, model.token_scores(before, tokens, top_k=top_k)
