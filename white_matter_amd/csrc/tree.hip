@@ -66,11 +66,11 @@ __device__ __forceinline__ tree_rsrc tree_buffer(const char* base, int bytes) {
   return __builtin_amdgcn_make_buffer_rsrc((void*)(((uint64_t)hi << 32) | lo), (short)0, __builtin_amdgcn_readfirstlane(bytes),
                                            0x00020000);
 }
-constexpr int kReadOnce = 2;  // cache policy: nontemporal
 
 // A value as if it changed here: what is derived from it (the lane masks of its
 // bits, a pair of scalar registers each) is formed at its use and not kept.
 __device__ __forceinline__ void fresh(uint32_t& x) { __asm__ volatile("" : "+v"(x)); }
+__device__ __forceinline__ void fresh(float& x) { __asm__ volatile("" : "+v"(x)); }
 
 struct TreeRange {
   int base;   // committed slots (every node sees them)
@@ -143,10 +143,13 @@ __device__ __forceinline__ f32x4 mfma16_half(const u32x4& a, const u32x4& b, con
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-
 // How a wave reads 32 slots of K and V.
-template <int FMT, int D>
+template <int FMT, int D, int MB>
 struct TreeTile {
+  // cache policy: nontemporal for slots read once; with two row blocks other row
+  // tiles, on the same XCD, read them too (64 nodes over 16 x 8,192 slots of e4m3:
+  // 102 us, 114 nontemporal; one token over 32 such rows 68 and 63)
+  static constexpr int kPolicy = MB == 1 ? 2 : 0;
   static constexpr int kElem = FMT == WMX_POOL_BF16 ? 2 : 1;  // bytes
   static constexpr int kRow = D * kElem;
   static constexpr int KS = D / 32;                           // k-steps of S^T
@@ -177,7 +180,7 @@ struct TreeTile {
       if constexpr (kWide) {
 #pragma unroll
         for (int j = 0; j < KS / 2; ++j) {
-          const auto w = __builtin_amdgcn_raw_buffer_load_b128(rs, off[u] + 64 * j, 0, kReadOnce);
+          const auto w = __builtin_amdgcn_raw_buffer_load_b128(rs, off[u] + 64 * j, 0, kPolicy);
 #pragma unroll
           for (int i = 0; i < 4; ++i) k[u][2 * j + i / 2][i % 2] = w[i];
         }
@@ -185,11 +188,11 @@ struct TreeTile {
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
           if constexpr (FMT == WMX_POOL_BF16) {
-            const auto w = __builtin_amdgcn_raw_buffer_load_b128(rs, off[u] + 64 * s, 0, kReadOnce);
+            const auto w = __builtin_amdgcn_raw_buffer_load_b128(rs, off[u] + 64 * s, 0, kPolicy);
 #pragma unroll
             for (int i = 0; i < 4; ++i) k[u][s][i] = w[i];
           } else {
-            const auto w = __builtin_amdgcn_raw_buffer_load_b64(rs, off[u] + 32 * s, 0, kReadOnce);
+            const auto w = __builtin_amdgcn_raw_buffer_load_b64(rs, off[u] + 32 * s, 0, kPolicy);
             k[u][s][0] = w[0];
             k[u][s][1] = w[1];
           }
@@ -204,22 +207,22 @@ struct TreeTile {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       if constexpr (FMT != WMX_POOL_BF16 && D == 96) {
-        v[e][0] = __builtin_amdgcn_raw_buffer_load_b32(rs, off[e], 0, kReadOnce);
-        v[e][1] = __builtin_amdgcn_raw_buffer_load_b16(rs, off[e] + 64 - 2 * li, 0, kReadOnce);
+        v[e][0] = __builtin_amdgcn_raw_buffer_load_b32(rs, off[e], 0, kPolicy);
+        v[e][1] = __builtin_amdgcn_raw_buffer_load_b16(rs, off[e] + 64 - 2 * li, 0, kPolicy);
       } else if constexpr (VD == 4) {
-        const auto w = __builtin_amdgcn_raw_buffer_load_b128(rs, off[e], 0, kReadOnce);
+        const auto w = __builtin_amdgcn_raw_buffer_load_b128(rs, off[e], 0, kPolicy);
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[e][i] = w[i];
       } else if constexpr (VD == 3) {
-        const auto w = __builtin_amdgcn_raw_buffer_load_b96(rs, off[e], 0, kReadOnce);
+        const auto w = __builtin_amdgcn_raw_buffer_load_b96(rs, off[e], 0, kPolicy);
 #pragma unroll
         for (int i = 0; i < 3; ++i) v[e][i] = w[i];
       } else if constexpr (VD == 2) {
-        const auto w = __builtin_amdgcn_raw_buffer_load_b64(rs, off[e], 0, kReadOnce);
+        const auto w = __builtin_amdgcn_raw_buffer_load_b64(rs, off[e], 0, kPolicy);
         v[e][0] = w[0];
         v[e][1] = w[1];
       } else {
-        v[e][0] = __builtin_amdgcn_raw_buffer_load_b32(rs, off[e], 0, kReadOnce);
+        v[e][0] = __builtin_amdgcn_raw_buffer_load_b32(rs, off[e], 0, kPolicy);
       }
     }
   }
@@ -265,7 +268,7 @@ __device__ __forceinline__ float sum_quarters(float x) {
 // One wave's state over its tiles, every kTreeWaves-th of its workgroup's.
 template <int FMT, int D, int MB>
 struct TreeWave {
-  using Tile = TreeTile<FMT, D>;
+  using Tile = TreeTile<FMT, D, MB>;
   static constexpr int KS = Tile::KS, W = Tile::W;
 
   u32x4 qf[MB][KS];  // queries, the B operand
@@ -288,26 +291,24 @@ struct TreeWave {
   int base, end;
   float scale;
 
+  // bytes of up to a tile's rows
   static __device__ __forceinline__ int span(int slots, int64_t step) {
-    return (int)((min(slots, kTreeTile) - 1) * step) + Tile::kRow;
+    return slots > 0 ? (int)((min(slots, kTreeTile) - 1) * step) + Tile::kRow : 0;
   }
   __device__ __forceinline__ void load_scales(int j0, const float* src, int q, float (&out)[8]) {
     if constexpr (FMT != WMX_POOL_BF16) {
-      typedef f32x4 f32x4_4 __attribute__((aligned(4)));
-      if (j0 + kTreeTile <= end) {
-        const f32x4 a = *(const f32x4_4*)(src + j0 + 4 * q), b = *(const f32x4_4*)(src + j0 + 16 + 4 * q);
+      const tree_rsrc rs = tree_buffer((const char*)(src + j0), 4 * max(0, min(end - j0, kTreeTile)));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          out[e] = a[e];
-          out[4 + e] = b[e];
-        }
-      } else {  // the last slot's for those behind it, which are masked
+      for (int u = 0; u < 2; ++u) {
+        const auto w = __builtin_amdgcn_raw_buffer_load_b128(rs, 16 * q + 64 * u, 0, 0);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) out[e] = src[min(j0 + Tile::key_of(q, e), end - 1)];
+        for (int i = 0; i < 4; ++i) out[4 * u + i] = __uint_as_float(w[i]);
       }
     }
   }
-  // slots past the last visible one read as zeros
+  // Slots past the last visible one read as zeros, and so does a tile past it: the
+  // loads of the next tile are issued without a branch around them, whose other
+  // side would make the waits for K wait for V as well.
   template <bool EDGE>
   __device__ __forceinline__ void load_k(int j0, int q) {
     tile.load_k(tree_buffer(kbase + j0 * ksb, span(end - j0, ksb)), koff);
@@ -377,7 +378,12 @@ struct TreeWave {
       // scores over the reference: the weights are exp2 of them
       float kq[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) kq[e] = FMT == WMX_POOL_BF16 ? scale : scale * ks[e];
+      for (int e = 0; e < 8; ++e) {
+        kq[e] = FMT == WMX_POOL_BF16 ? scale : scale * ks[e];
+        // formed here: K's scales of the next tile are loaded into the same
+        // registers, and not into others whose copying waits for all loads
+        if constexpr (FMT != WMX_POOL_BF16) fresh(kq[e]);
+      }
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb) {
 #pragma unroll
@@ -385,7 +391,7 @@ struct TreeWave {
       }
     }
     const int next = j0 + kTreeStep;
-    if (next < end) load_k<EDGE>(next, q);  // K's registers are free
+    load_k<EDGE>(next, q);  // K's registers are free
 
     if constexpr (EDGE) {
 #pragma unroll
@@ -397,10 +403,13 @@ struct TreeWave {
     }
 
     if constexpr (FMT != WMX_POOL_BF16) {
-      float most = 0.f;  // (NaN stays out of it, and an infinity)
+      float most = 0.f;  // (NaN stays out of it)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(vs[e]) < kPosInf ? fabsf(vs[e]) : 0.f);
+      for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(vs[e]));
       if (__any(most * vref > kScaleRoom)) {
+        most = 0.f;  // (and here an infinity)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) most = fmaxf(most, fabsf(vs[e]) < kPosInf ? fabsf(vs[e]) : 0.f);
         const float to = scale_lv(most), f = __builtin_amdgcn_exp2f(to - lv);
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb) {
@@ -492,7 +501,7 @@ struct TreeWave {
         }
       }
     }
-    if (next < end) load_v(next, q, li);
+    load_v(next, q, li);
   }
 };
 
@@ -535,9 +544,9 @@ __device__ __forceinline__ TreePartials tree_partials(const wmx_tree_args& a, co
 }
 
 template <int FMT, int D, int MB>
-__global__ __launch_bounds__(64 * kTreeWaves, (MB == 1 && TreeTile<FMT, D>::kRow < 256) ? 3 : 2) void tree_kernel(
+__global__ __launch_bounds__(64 * kTreeWaves, (MB == 1 && TreeTile<FMT, D, MB>::kRow < 256) ? 3 : 2) void tree_kernel(
     const wmx_tree_args a, const TreeLaunch t) {
-  using Tile = TreeTile<FMT, D>;
+  using Tile = TreeTile<FMT, D, MB>;
   constexpr int KS = Tile::KS, W = Tile::W, ROWS = 16 * MB;
   constexpr int LDR = 4 * W + 4;  // LDS row of one merge round: four quarters x W, padded against bank conflicts
   __shared__ __attribute__((aligned(16))) float lds_o[kTreeWaves][ROWS][LDR];
