@@ -21,6 +21,7 @@
 // of one per element. Codes are converted exactly: K's to bf16 like the
 // queries; V's to fp16, in which the weights keep 11 bits (bf16 pools: 8).
 #include <climits>
+#include "lds_tiles.h"
 #include "wmx_kernels.h"
 
 namespace wmx {
@@ -57,20 +58,6 @@ __device__ __forceinline__ uint32_t code_pair_half(uint32_t w) {
     return __builtin_bit_cast(uint32_t, x);
   }
 }
-
-typedef __amdgpu_buffer_rsrc_t tree_rsrc;
-// A raw buffer over [base, base + bytes), both wave-uniform; reads past it give zeros.
-__device__ __forceinline__ tree_rsrc tree_buffer(const char* base, int bytes) {
-  const uint64_t p = (uint64_t)base;
-  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)p), hi = __builtin_amdgcn_readfirstlane((uint32_t)(p >> 32));
-  return __builtin_amdgcn_make_buffer_rsrc((void*)(((uint64_t)hi << 32) | lo), (short)0, __builtin_amdgcn_readfirstlane(bytes),
-                                           0x00020000);
-}
-
-// A value as if it changed here: what is derived from it (the lane masks of its
-// bits, a pair of scalar registers each) is formed at its use and not kept.
-__device__ __forceinline__ void fresh(uint32_t& x) { __asm__ volatile("" : "+v"(x)); }
-__device__ __forceinline__ void fresh(float& x) { __asm__ volatile("" : "+v"(x)); }
 
 struct TreeRange {
   int base;   // committed slots (every node sees them)
@@ -174,13 +161,36 @@ struct TreeTile {
   uint32_t k[2][KS][KD];  // key halves
   uint32_t v[8][VD];      // the lane's keys
 
-  __device__ __forceinline__ void load_k(const tree_rsrc& rs, const int (&off)[2]) {
+  // K goes through LDS: lanes next to each other load chunks of 16 bytes next to
+  // each other, which the L1 serves a line at a time, where the operand's lanes
+  // are rows, and 64 lines an instruction. Chunk c of row r is stored as chunk
+  // c ^ k_swizzle(r) (D = 96 by pairs or fours), so that 16 rows' chunks c lie in
+  // different banks.
+  static constexpr int kChunks = kRow / 16, kLoads = kTreeTile * kChunks / 64;
+  static __device__ __forceinline__ int k_swizzle(int r) {
+    if constexpr (kRow == 192) return (r >> 2) & 3;
+    else if constexpr (kRow == 96) return (r >> 3) & 1;
+    else return (r / (256 / kRow)) & (kChunks - 1);
+  }
+  // byte offset of what lane `lane` loads with instruction i
+  static __device__ __forceinline__ int k_source(int lane, int i, int step) {
+    const int g = 64 * i + lane, r = g / kChunks;
+    return r * step + 16 * ((g - r * kChunks) ^ k_swizzle(r));
+  }
+  static __device__ __forceinline__ void stage_k(const rsrc_t& rs, char* stage, const int (&off)[kLoads]) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (lds_void*)(stage + 1024 * i), 16, off[i], 0, 0, kPolicy);
+  }
+  __device__ __forceinline__ void read_k(const char* stage, int li, int q) {
+    const int swz = k_swizzle(li);  // (rows 16 apart share it)
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
+      const char* row = stage + (16 * u + li) * kRow;
       if constexpr (kWide) {
 #pragma unroll
         for (int j = 0; j < KS / 2; ++j) {
-          const auto w = __builtin_amdgcn_raw_buffer_load_b128(rs, off[u] + 64 * j, 0, kPolicy);
+          const u32x4 w = *(const u32x4*)(row + 16 * ((q + 4 * j) ^ swz));
 #pragma unroll
           for (int i = 0; i < 4; ++i) k[u][2 * j + i / 2][i % 2] = w[i];
         }
@@ -188,11 +198,11 @@ struct TreeTile {
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
           if constexpr (FMT == WMX_POOL_BF16) {
-            const auto w = __builtin_amdgcn_raw_buffer_load_b128(rs, off[u] + 64 * s, 0, kPolicy);
+            const u32x4 w = *(const u32x4*)(row + 16 * ((q + 4 * s) ^ swz));
 #pragma unroll
             for (int i = 0; i < 4; ++i) k[u][s][i] = w[i];
           } else {
-            const auto w = __builtin_amdgcn_raw_buffer_load_b64(rs, off[u] + 32 * s, 0, kPolicy);
+            const u32x2 w = *(const u32x2*)(row + 16 * (((q >> 1) + 2 * s) ^ swz) + 8 * (q & 1));
             k[u][s][0] = w[0];
             k[u][s][1] = w[1];
           }
@@ -200,10 +210,8 @@ struct TreeTile {
       }
     }
   }
-  // byte offset of the lane's K part in a row
-  static __device__ __forceinline__ int k_part(int q) { return kWide || FMT == WMX_POOL_BF16 ? 16 * q : 8 * q; }
 
-  __device__ __forceinline__ void load_v(const tree_rsrc& rs, const int (&off)[8], int li) {
+  __device__ __forceinline__ void load_v(const rsrc_t& rs, const int (&off)[8], int li) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       if constexpr (FMT != WMX_POOL_BF16 && D == 96) {
@@ -277,7 +285,8 @@ struct TreeWave {
   float lv, vref;    // (vref = 2^lv)
   Tile tile;
   float ks[8], vs[8];
-  int koff[2], voff[8];
+  int koff[Tile::kLoads], voff[8];
+  char* stage;       // this wave's K tile in LDS, and behind it the K and V scales of its slots
   uint32_t kept[8];  // key_mask of the lane's keys
   bool odd;          // this lane met a drafted value that is not finite
 
@@ -295,14 +304,25 @@ struct TreeWave {
   static __device__ __forceinline__ int span(int slots, int64_t step) {
     return slots > 0 ? (int)((min(slots, kTreeTile) - 1) * step) + Tile::kRow : 0;
   }
-  __device__ __forceinline__ void load_scales(int j0, const float* src, int q, float (&out)[8]) {
+  static constexpr int kTileBytes = kTreeTile * Tile::kRow;
+  // 32 K scales, 32 V scales: half the lanes load zeros past them
+  __device__ __forceinline__ void stage_scales(int j0, int lane) {
     if constexpr (FMT != WMX_POOL_BF16) {
-      const tree_rsrc rs = tree_buffer((const char*)(src + j0), 4 * max(0, min(end - j0, kTreeTile)));
+      const int bytes = 4 * max(0, min(end - j0, kTreeTile));
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(make_rsrc(kscale + j0, bytes), (lds_void*)(stage + kTileBytes), 4, 4 * lane, 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(make_rsrc(vscale + j0, bytes), (lds_void*)(stage + kTileBytes + 256), 4, 4 * lane, 0, 0, 0);
+    }
+  }
+  __device__ __forceinline__ void read_scales(int q) {
+    if constexpr (FMT != WMX_POOL_BF16) {
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const auto w = __builtin_amdgcn_raw_buffer_load_b128(rs, 16 * q + 64 * u, 0, 0);
+        const f32x4 a = *(const f32x4*)(stage + kTileBytes + 16 * q + 64 * u), b = *(const f32x4*)(stage + kTileBytes + 256 + 16 * q + 64 * u);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) out[4 * u + i] = __uint_as_float(w[i]);
+        for (int i = 0; i < 4; ++i) {
+          ks[4 * u + i] = a[i];
+          vs[4 * u + i] = b[i];
+        }
       }
     }
   }
@@ -310,18 +330,17 @@ struct TreeWave {
   // loads of the next tile are issued without a branch around them, whose other
   // side would make the waits for K wait for V as well.
   template <bool EDGE>
-  __device__ __forceinline__ void load_k(int j0, int q) {
-    tile.load_k(tree_buffer(kbase + j0 * ksb, span(end - j0, ksb)), koff);
-    load_scales(j0, kscale, q, ks);
+  __device__ __forceinline__ void load_k(int j0, int lane, int q) {
+    Tile::stage_k(make_rsrc(kbase + j0 * ksb, span(end - j0, ksb)), stage, koff);
+    stage_scales(j0, lane);
     if (EDGE && kmask) {  // (zero past the last slot; with a key mask every tile is an edge)
-      const tree_rsrc rs = tree_buffer((const char*)kmask, end);
+      const rsrc_t rs = make_rsrc(kmask, end);
 #pragma unroll
       for (int e = 0; e < 8; ++e) kept[e] = __builtin_amdgcn_raw_buffer_load_b8(rs, j0 + Tile::key_of(q, e), 0, 0);
     }
   }
   __device__ __forceinline__ void load_v(int j0, int q, int li) {
-    tile.load_v(tree_buffer(vbase + j0 * vsb, span(end - j0, vsb)), voff, li);
-    load_scales(j0, vscale, q, vs);
+    tile.load_v(make_rsrc(vbase + j0 * vsb, span(end - j0, vsb)), voff, li);
   }
 
   // One tile. EDGE: some of its slots are masked, drafted or past the end.
@@ -338,7 +357,7 @@ struct TreeWave {
         const int j = j0 + Tile::key_of(q, e);
         const bool ok = j < end && (!kmask || kept[e] != 0);
         keep[e] = ok ? ~0u : 0u;
-        fresh(keep[e]);
+        opaque(keep[e]);
         kept_bits |= (ok ? 1u : 0u) << e;
         drafted |= (ok && j >= base ? 1u : 0u) << e;
       }
@@ -346,11 +365,11 @@ struct TreeWave {
       for (int mb = 0; mb < MB; ++mb) seen[mb] = kept_bits;
       if (any_drafted) {
         // (a query's bytes past the last slot and before the first drafted one are not read)
-        const tree_rsrc rs = tree_buffer((const char*)tmask, tree_bytes);
+        const rsrc_t rs = make_rsrc(tmask, tree_bytes);
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb) {
           uint32_t t[8];
-          fresh(drafted);
+          opaque(drafted);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const int a = j0 + Tile::key_of(q, e) - base;
@@ -361,6 +380,13 @@ struct TreeWave {
         }
       }
     }
+    // K and the scales go to registers, and the next tile's into their place
+    const int next = j0 + kTreeStep, lane = 16 * q + li;
+    tile.read_k(stage, li, q);
+    read_scales(q);
+    lgkm_settle();
+    load_k<EDGE>(next, lane, q);
+
     float sc[MB][8];
     {
       f32x4 s[MB][2];
@@ -378,25 +404,18 @@ struct TreeWave {
       // scores over the reference: the weights are exp2 of them
       float kq[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        kq[e] = FMT == WMX_POOL_BF16 ? scale : scale * ks[e];
-        // formed here: K's scales of the next tile are loaded into the same
-        // registers, and not into others whose copying waits for all loads
-        if constexpr (FMT != WMX_POOL_BF16) fresh(kq[e]);
-      }
+      for (int e = 0; e < 8; ++e) kq[e] = FMT == WMX_POOL_BF16 ? scale : scale * ks[e];
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) sc[mb][e] = fmaf(s[mb][e >> 2][e & 3], kq[e], -row[mb].ref);
       }
     }
-    const int next = j0 + kTreeStep;
-    load_k<EDGE>(next, q);  // K's registers are free
 
     if constexpr (EDGE) {
 #pragma unroll
       for (int mb = 0; mb < MB; ++mb) {
-        fresh(seen[mb]);
+        opaque(seen[mb]);
 #pragma unroll
         for (int e = 0; e < 8; ++e) sc[mb][e] = (seen[mb] >> e) & 1u ? sc[mb][e] : kNegInf;
       }
@@ -439,7 +458,7 @@ struct TreeWave {
         for (int e = 0; e < 8; ++e) sc[mb][e] -= up;
       }
       float x[8];
-      if constexpr (EDGE) fresh(seen[mb]);
+      if constexpr (EDGE) opaque(seen[mb]);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         x[e] = __builtin_amdgcn_exp2f(sc[mb][e]);
@@ -473,7 +492,7 @@ struct TreeWave {
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] &= keep[e];
         if (any_drafted) {
-          fresh(drafted);
+          opaque(drafted);
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             const bool draft = (drafted >> e) & 1u;
@@ -550,6 +569,7 @@ __global__ __launch_bounds__(64 * kTreeWaves, (MB == 1 && TreeTile<FMT, D, MB>::
   constexpr int KS = Tile::KS, W = Tile::W, ROWS = 16 * MB;
   constexpr int LDR = 4 * W + 4;  // LDS row of one merge round: four quarters x W, padded against bank conflicts
   __shared__ __attribute__((aligned(16))) float lds_o[kTreeWaves][ROWS][LDR];
+  __shared__ __attribute__((aligned(16))) char stage[kTreeWaves][TreeWave<FMT, D, MB>::kTileBytes + (FMT == WMX_POOL_BF16 ? 0 : 512)];
   __shared__ float lds_m[kTreeWaves][ROWS], lds_l[kTreeWaves][ROWS], lds_max[ROWS], lds_sum[ROWS];
   __shared__ int lds_odd, lds_wave[kTreeWaves], lds_all[kTreeWaves], lds_first[4];
 
@@ -657,10 +677,11 @@ __global__ __launch_bounds__(64 * kTreeWaves, (MB == 1 && TreeTile<FMT, D, MB>::
     w.end = end;
     w.scale = a.softmax_scale * kLog2e;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) w.koff[u] = (16 * u + li) * (int)w.ksb + Tile::k_part(q);
+    for (int i = 0; i < Tile::kLoads; ++i) w.koff[i] = Tile::k_source(lane, i, (int)w.ksb);
+    w.stage = stage[wave];
 #pragma unroll
     for (int e = 0; e < 8; ++e) w.voff[e] = Tile::key_of(q, e) * (int)vsb + Tile::v_part(li);
-    w.template load_k<true>(j0, q);
+    w.template load_k<true>(j0, lane, q);
     w.load_v(j0, q, li);
     // this lane's queries: rows row0 + 16 mb + li (zeros past the last)
 #pragma unroll
@@ -680,6 +701,7 @@ __global__ __launch_bounds__(64 * kTreeWaves, (MB == 1 && TreeTile<FMT, D, MB>::
     const int whole = kmask ? begin : min(range.base, end);  // slots that every query sees end here
     for (; j0 + kTreeTile <= whole; j0 += kTreeStep) w.template step<false>(j0, li, q);
     for (; j0 < end; j0 += kTreeStep) w.template step<true>(j0, li, q);
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the last loads into LDS (zeros, of a tile past the end) are done
   }
 
   // the workgroup's waves merged: maxima and sums, then the outputs in four
