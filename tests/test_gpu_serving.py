@@ -362,13 +362,15 @@ def test_tree_attention_padded_head_dim():
 
 @pytest.mark.parametrize("kind", ["bf16", "e4m3", "int8"])
 @pytest.mark.parametrize(("batch", "heads", "kv_heads", "nodes"), [(1, 2, 1, 1), (6, 4, 2, 1), (6, 4, 2, 19), (70, 2, 1, 3), (256, 1, 1, 1), (257, 1, 1, 1)])
+@pytest.mark.parametrize("capacity", [1700, 5200])
 @torch.no_grad()
-def test_tree_attention_deals_ragged_batches(kind, batch, heads, kv_heads, nodes):
-    """Pools long enough for work dealt out by the lengths: most rows short, some
-    empty, few long, with and without a key mask that leaves ranges empty; the
-    same launch captured, and replayed after the lengths have changed."""
-    print(f"dealt {kind} B={batch} H={heads}/{kv_heads} n={nodes}", flush=True)
-    gen, capacity, dim = _gen(batch + nodes), 1700, 64
+def test_tree_attention_deals_ragged_batches(kind, capacity, batch, heads, kv_heads, nodes):
+    """Pools of one range a row, and long enough for work dealt out by the
+    lengths: most rows short, some empty, few long, with and without a key mask
+    that leaves ranges empty; the same launch captured, and replayed after the
+    lengths have changed."""
+    print(f"dealt {kind} N={capacity} B={batch} H={heads}/{kv_heads} n={nodes}", flush=True)
+    gen, dim = _gen(batch + nodes), 64
     key, value, k, v = _pool_pair(gen, (batch, kv_heads, capacity, dim), kind)
     query = _randn(gen, batch, heads, nodes, dim)
     tree = _random_tree(gen, batch, nodes)

@@ -4,14 +4,16 @@
 // The query rows of one KV head (nodes x query heads of its group, node-major)
 // share its keys and values, so a workgroup takes 16 MB of them and a range of
 // slots; each K/V byte is read from HBM once per row tile and converted once.
-// Four waves take every fourth 32-slot tile of the range and keep their own
-// running maximum, sum and output, merged through LDS at the end; ranges of
-// one row are merged by a second kernel in log-sum-exp form.
+// Four waves (eight where there are few workgroups) take turns at the range's
+// 32-slot tiles and keep their own running maximum, sum and output, merged
+// through LDS at the end; ranges of one row are merged by a second kernel in
+// log-sum-exp form.
 //
-// Nothing is staged in LDS: with v_mfma_f32_16x16x32_bf16
+// With v_mfma_f32_16x16x32_bf16
 //   S^T = K Q^T    A: lane l holds key l % 16, 8 consecutive d of its quarter
-//                  l / 16; the d order is the one in which its loads are
-//                  widest, the same for Q
+//                  l / 16; the d order is the one in which its reads are
+//                  widest, the same for Q. K tiles pass through LDS (see
+//                  k_swizzle), and the scales with them
 //   O^T = V^T P^T  B: P as S^T left it in the accumulators: lane (query l % 16,
 //                  quarter q) holds keys 4 q + [0, 4) of the tile's two
 //                  16-key halves; A: V of those keys, loaded as D/16
@@ -119,9 +121,7 @@ __device__ __forceinline__ float scale_lv(float most) {
 }
 constexpr float kScaleStart = 100.f;
 
-constexpr int kTreeWaves = 4;
 constexpr int kTreeTile = 32;                      // slots per wave and step
-constexpr int kTreeStep = kTreeWaves * kTreeTile;  // slots per workgroup and step
 
 __device__ __forceinline__ f32x4 mfma16(const u32x4& a, const u32x4& b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(a), as_bf16x8(b), c, 0, 0, 0);
@@ -163,9 +163,10 @@ struct TreeTile {
 
   // K goes through LDS: lanes next to each other load chunks of 16 bytes next to
   // each other, which the L1 serves a line at a time, where the operand's lanes
-  // are rows, and 64 lines an instruction. Chunk c of row r is stored as chunk
-  // c ^ k_swizzle(r) (D = 96 by pairs or fours), so that 16 rows' chunks c lie in
-  // different banks.
+  // are rows, and 64 lines an instruction (64 nodes over 16 rows of up to 8,192
+  // slots: 86 us, 102 with the operands loaded directly). Chunk c of row r is
+  // stored as chunk c ^ k_swizzle(r) (D = 96 by pairs or fours), so that 16 rows'
+  // chunks c lie in different banks.
   static constexpr int kChunks = kRow / 16, kLoads = kTreeTile * kChunks / 64;
   static __device__ __forceinline__ int k_swizzle(int r) {
     if constexpr (kRow == 192) return (r >> 2) & 3;
@@ -256,11 +257,11 @@ struct TreeTile {
 };
 
 // Steps of a batch row, per KV head (one at least: its outputs are written).
-__device__ __forceinline__ int tree_steps(const wmx_tree_args& a, int b) {
+__device__ __forceinline__ int tree_steps(const wmx_tree_args& a, int b, int step) {
   int64_t len = a.kv_lengths ? a.kv_lengths[b] : a.kv_length_scalar;
   len = len < 0 ? 0 : len > a.capacity ? a.capacity : len + a.use_dummy;
   const int64_t total = min(a.tree_mask ? len + a.nodes : len, (int64_t)a.capacity);
-  return max(1, (int)((total + kTreeStep - 1) / kTreeStep));
+  return max(1, (int)((total + step - 1) / step));
 }
 
 // x of lanes l ^ 16 and l ^ 32 joined with this lane's, the same in all four
@@ -273,8 +274,8 @@ __device__ __forceinline__ float sum_quarters(float x) {
   return sum_halves(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
-// One wave's state over its tiles, every kTreeWaves-th of its workgroup's.
-template <int FMT, int D, int MB>
+// One wave's state over its tiles, every NW-th of its workgroup's.
+template <int FMT, int D, int MB, int NW>
 struct TreeWave {
   using Tile = TreeTile<FMT, D, MB>;
   static constexpr int KS = Tile::KS, W = Tile::W;
@@ -381,7 +382,7 @@ struct TreeWave {
       }
     }
     // K and the scales go to registers, and the next tile's into their place
-    const int next = j0 + kTreeStep, lane = 16 * q + li;
+    const int next = j0 + NW * kTreeTile, lane = 16 * q + li;
     tile.read_k(stage, li, q);
     read_scales(q);
     lgkm_settle();
@@ -525,28 +526,34 @@ struct TreeWave {
 };
 
 // Which key range a workgroup takes. The slots of every (batch row, KV head), the
-// drafted ones included, are counted in steps of kTreeStep. With nsplit 0 the
-// workgroups are dealt out by these counts: all steps over `ranges` give a share,
-// a (row, head) of n steps gets ceil(n / share) workgroups, and these split its
-// steps evenly; a row of one writes the outputs itself. Rows of any lengths then
-// load the card alike, whatever the pool's capacity. With nsplit > 0 every (row,
-// head) has that many ranges of `share` steps.
+// drafted ones included, are counted in steps of a workgroup (32 per wave). With
+// nsplit 0 the workgroups are dealt out by these counts: all steps over `share`
+// workgroups give a part, a (row, head) of n steps gets ceil(n / part) workgroups,
+// and these split its steps evenly; a row of one writes the outputs itself. Rows
+// of any lengths then load the card alike, whatever the pool's capacity. With
+// nsplit > 0 every (row, head) has that many ranges of `share` steps.
 struct TreeLaunch {
-  int tiles, ranges, nsplit, share;
+  int tiles, ranges, nsplit, share, waves;
 };
-// Pools of up to so many steps (1,280 slots) are not split: the second launch and
-// the partials cost more than idle CUs do (600 slots: 8 rows of one node 12 us,
-// 16 us dealt; 32 rows of 64 nodes 30 and 36. 1,280 slots: 10.0 and 13.5 us for a
-// row, 8 rows of 16 nodes 19.2 and 17.2. 2,500 slots: 16.5 and 14.2 us for a row,
-// 8 rows 25 and 17).
-constexpr int kOneRange = 10;
+// One range a row, in one launch, for pools of up to so many slots, and of twice
+// as many where the rows' workgroups fill the CUs: the second launch, the partials
+// and the dealing cost more than idle CUs do. Up to a workgroup a CU, eight waves
+// share the row's slots. Us, one range and dealt, e4m3, 8 KV heads of two queries:
+// 1,153 slots, one token over one row (D 64) 9 and 13; 1,700 slots (D 128) one row
+// 11 and 14, 8 rows 15 and 17, 64 nodes over 8 rows 22 and 30; 2,500 slots, 4
+// rows 17 and 17, 8 rows 20 and 17.5, 32 rows 23.5 and 30. 3,500 slots, 4 rows 22
+// and 17, but 32 rows 30 and 35, 16 nodes 32 and 42; 4,800 slots, 32 rows 36 and
+// 38.5. Eight waves and four: 16 nodes over 8 rows of 1,280 slots 17.3 and 19.1,
+// with more than a workgroup a CU 64 nodes over 32 rows of 1,700 slots 70 and 54.
+constexpr int kOneRange = 2560, kCUs = 256;
 constexpr int kPlanRows = 256;  // most batch rows whose workgroups are dealt out
 // How the steps are dealt, by the query rows of a workgroup: 16 rows stream the
 // slots, and four workgroups a CU, of at least four steps, are best (e4m3, D 128,
-// 8 KV heads, up to 8,192 slots: 32 rows 68 us, 71 with two a CU, 75 with twelve;
-// 8 rows 27 us, 32 with workgroups of two steps). With 32 rows the arithmetic sets
-// the pace: one a CU, of any length (64 nodes over 16 x 8,192 slots 119 us, 124
-// with two a CU; 4 x 1,500 slots 14 us, 17 with four steps at least).
+// 8 KV heads, up to 8,192 slots, one token: 32 rows 58.5 us, 60 with two a CU, 61
+// with eight; 8 rows 24 us, 29 with workgroups of two steps). With 32 rows the
+// arithmetic sets the pace: one a CU, of any length (64 nodes over 16 such rows 85
+// us, 92 with two a CU; 13 nodes over 4 bf16 rows of 4,096 slots 21, 23, with
+// four a CU 29).
 __host__ __device__ constexpr int tree_dealt(int rows) { return rows == 16 ? 1024 : 256; }
 __host__ __device__ constexpr int tree_min_share(int rows) { return rows == 16 ? 4 : 1; }
 // At the workspace's start, for the merge: the ranges before each row (per KV head), and all.
@@ -562,16 +569,16 @@ __device__ __forceinline__ TreePartials tree_partials(const wmx_tree_args& a, co
   return TreePartials{o + tree_partial_rows(t, rows) * a.head_dim, o};
 }
 
-template <int FMT, int D, int MB>
-__global__ __launch_bounds__(64 * kTreeWaves, (MB == 1 && TreeTile<FMT, D, MB>::kRow < 256) ? 3 : 2) void tree_kernel(
+template <int FMT, int D, int MB, int NW>
+__global__ __launch_bounds__(64 * NW, (NW == 4 && MB == 1 && TreeTile<FMT, D, MB>::kRow < 256) ? 3 : 2) void tree_kernel(
     const wmx_tree_args a, const TreeLaunch t) {
   using Tile = TreeTile<FMT, D, MB>;
-  constexpr int KS = Tile::KS, W = Tile::W, ROWS = 16 * MB;
+  constexpr int KS = Tile::KS, W = Tile::W, ROWS = 16 * MB, STEP = NW * kTreeTile;
   constexpr int LDR = 4 * W + 4;  // LDS row of one merge round: four quarters x W, padded against bank conflicts
-  __shared__ __attribute__((aligned(16))) float lds_o[kTreeWaves][ROWS][LDR];
-  __shared__ __attribute__((aligned(16))) char stage[kTreeWaves][TreeWave<FMT, D, MB>::kTileBytes + (FMT == WMX_POOL_BF16 ? 0 : 512)];
-  __shared__ float lds_m[kTreeWaves][ROWS], lds_l[kTreeWaves][ROWS], lds_max[ROWS], lds_sum[ROWS];
-  __shared__ int lds_odd, lds_wave[kTreeWaves], lds_all[kTreeWaves], lds_first[4];
+  __shared__ __attribute__((aligned(16))) float lds_o[NW][ROWS][LDR];
+  __shared__ __attribute__((aligned(16))) char stage[NW][TreeWave<FMT, D, MB, NW>::kTileBytes + (FMT == WMX_POOL_BF16 ? 0 : 512)];
+  __shared__ float lds_m[NW][ROWS], lds_l[NW][ROWS], lds_max[ROWS], lds_sum[ROWS];
+  __shared__ int lds_odd, lds_wave[NW], lds_all[NW], lds_first[4];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = wave_id();
   const int li = lane & 15, q = lane >> 4;
@@ -593,7 +600,7 @@ __global__ __launch_bounds__(64 * kTreeWaves, (MB == 1 && TreeTile<FMT, D, MB>::
     s1 = s0 + t.share;
     parts = t.nsplit;
   } else {
-    const int steps = tid < a.batch ? tree_steps(a, tid) : 0;
+    const int steps = tid < a.batch ? tree_steps(a, tid, STEP) : 0;
     int sum = steps;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) sum += __shfl_xor(sum, o);
@@ -601,7 +608,7 @@ __global__ __launch_bounds__(64 * kTreeWaves, (MB == 1 && TreeTile<FMT, D, MB>::
     __syncthreads();
     int all = 0;
 #pragma unroll
-    for (int i = 0; i < kTreeWaves; ++i) all += lds_wave[i];
+    for (int i = 0; i < NW; ++i) all += lds_wave[i];
     const int share = max(tree_min_share(ROWS), (all * a.kv_heads + t.share - 1) / t.share);
     const int n = (steps + share - 1) / share;
     int before = n;  // inclusive scan over the workgroup
@@ -614,7 +621,7 @@ __global__ __launch_bounds__(64 * kTreeWaves, (MB == 1 && TreeTile<FMT, D, MB>::
     __syncthreads();
     int ranges = 0;
 #pragma unroll
-    for (int i = 0; i < kTreeWaves; ++i) {
+    for (int i = 0; i < NW; ++i) {
       before += i < wave ? lds_all[i] : 0;
       ranges += lds_all[i];
     }
@@ -642,14 +649,14 @@ __global__ __launch_bounds__(64 * kTreeWaves, (MB == 1 && TreeTile<FMT, D, MB>::
   }
   const TreeRange range = tree_range(a, b);
   const bool complete = parts == 1;
-  const int begin = min(s0 * kTreeStep, range.total), end = min(s1 * kTreeStep, range.total);
+  const int begin = min(s0 * STEP, range.total), end = min(s1 * STEP, range.total);
   const uint8_t* kmask = a.key_mask ? a.key_mask + (int64_t)b * a.key_mask_stride : nullptr;
   const uint8_t* tmask = a.tree_mask ? a.tree_mask + (int64_t)b * a.tree_mask_stride[0] : nullptr;
   const char* vbase = (const char*)a.v + ((int64_t)b * a.v_stride[0] + (int64_t)hk * a.v_stride[1]) * Tile::kElem;
   const int64_t vsb = a.v_stride[2] * Tile::kElem;
   if (tid == 0) lds_odd = 0;
 
-  TreeWave<FMT, D, MB> w;
+  TreeWave<FMT, D, MB, NW> w;
   w.lv = FMT == WMX_POOL_BF16 ? 0.f : kScaleStart;
   w.vref = __builtin_amdgcn_exp2f(w.lv);
   w.odd = false;
@@ -699,8 +706,8 @@ __global__ __launch_bounds__(64 * kTreeWaves, (MB == 1 && TreeTile<FMT, D, MB>::
       }
     }
     const int whole = kmask ? begin : min(range.base, end);  // slots that every query sees end here
-    for (; j0 + kTreeTile <= whole; j0 += kTreeStep) w.template step<false>(j0, li, q);
-    for (; j0 < end; j0 += kTreeStep) w.template step<true>(j0, li, q);
+    for (; j0 + kTreeTile <= whole; j0 += STEP) w.template step<false>(j0, li, q);
+    for (; j0 < end; j0 += STEP) w.template step<true>(j0, li, q);
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the last loads into LDS (zeros, of a tile past the end) are done
   }
 
@@ -722,9 +729,9 @@ __global__ __launch_bounds__(64 * kTreeWaves, (MB == 1 && TreeTile<FMT, D, MB>::
   if (tid < ROWS) {
     float mx = lds_m[0][tid], sum = 0.f;
 #pragma unroll
-    for (int i = 1; i < kTreeWaves; ++i) mx = fmaxf(mx, lds_m[i][tid]);
+    for (int i = 1; i < NW; ++i) mx = fmaxf(mx, lds_m[i][tid]);
 #pragma unroll
-    for (int i = 0; i < kTreeWaves; ++i) {
+    for (int i = 0; i < NW; ++i) {
       // (a wave that saw nothing has the sum 0, a row of NaN scores no maximum)
       const float f = lds_m[i][tid] == kNegInf ? 1.f : __builtin_amdgcn_exp2f(lds_m[i][tid] - mx);
       sum += lds_l[i][tid] == 0.f ? 0.f : lds_l[i][tid] * f;
@@ -764,13 +771,13 @@ __global__ __launch_bounds__(64 * kTreeWaves, (MB == 1 && TreeTile<FMT, D, MB>::
         }
       }
       __syncthreads();
-      for (int i = tid; i < PAIRS; i += 64 * kTreeWaves) {
+      for (int i = tid; i < PAIRS; i += 64 * NW) {
         const int row = i / (2 * W), x = i - row * 2 * W;
         const int qq = x / (W / 2), c = 2 * (x - qq * (W / 2));
         if (row0 + row >= rows) continue;
         float o0 = 0.f, o1 = 0.f;
 #pragma unroll
-        for (int i4 = 0; i4 < kTreeWaves; ++i4) {
+        for (int i4 = 0; i4 < NW; ++i4) {
           o0 += lds_o[i4][row][W * qq + c];
           o1 += lds_o[i4][row][W * qq + c + 1];
         }
@@ -875,21 +882,20 @@ static int tree_rows(const wmx_tree_args& a) { return (int64_t)a.nodes * (a.q_he
 static TreeLaunch tree_plan(const wmx_tree_args& a) {
   const int64_t rows = (int64_t)a.nodes * (a.q_heads / a.kv_heads), per = tree_rows(a);
   const int64_t tiles = (rows + per - 1) / per, pairs = (int64_t)a.batch * a.kv_heads;
-  const int64_t most = max(1, (a.capacity + kTreeStep - 1) / kTreeStep);  // steps of a (row, head)
   TreeLaunch t{};
   t.tiles = (int)tiles;
-  if (a.num_splits > 0) {
-    t.nsplit = a.num_splits;
-  } else if (most <= kOneRange || a.batch > kPlanRows || pairs * most > (1 << 30)) {
-    t.nsplit = 1;
+  const bool few = a.capacity <= kOneRange || (a.capacity <= 2 * kOneRange && pairs * tiles >= kCUs);
+  t.nsplit = a.num_splits > 0 ? a.num_splits : few || a.batch > kPlanRows || pairs * a.capacity > (1ll << 36) ? 1 : 0;
+  t.waves = t.nsplit == 1 && pairs * tiles <= kCUs ? 8 : 4;
+  const int64_t step = t.waves * kTreeTile, most = max((int64_t)1, (a.capacity + step - 1) / step);  // steps of a (row, head)
+  if (t.nsplit > 0) {
+    t.share = (int)((most + t.nsplit - 1) / t.nsplit);
+    t.ranges = (int)min((int64_t)INT32_MAX, pairs * t.nsplit);
   } else {
     const int64_t least = tree_min_share((int)per);
     t.share = (int)max((int64_t)1, tree_dealt((int)per) / tiles);  // workgroups to deal the steps over
     t.ranges = (int)min(pairs + t.share, pairs * ((most + least - 1) / least));
-    return t;
   }
-  t.share = (int)((most + t.nsplit - 1) / t.nsplit);
-  t.ranges = (int)min((int64_t)INT32_MAX, pairs * t.nsplit);
   return t;
 }
 
@@ -898,19 +904,19 @@ int64_t tree_workspace_size(const wmx_tree_args& a) {
   return t.nsplit == 1 ? 0 : 4 * (kPlanInts + tree_partial_rows(t, tree_rows(a)) * (a.head_dim + 2));
 }
 
-template <int FMT, int D>
+template <int FMT, int D, int MB>
 static void launch_tree_d(const wmx_tree_args& a, unsigned blocks, const TreeLaunch& t, hipStream_t stream) {
-  const dim3 grid(blocks), block(64 * kTreeWaves);
-  if (tree_rows(a) == 16) hipLaunchKernelGGL((tree_kernel<FMT, D, 1>), grid, block, 0, stream, a, t);
-  else hipLaunchKernelGGL((tree_kernel<FMT, D, 2>), grid, block, 0, stream, a, t);
+  const dim3 grid(blocks), block(64 * t.waves);
+  if (t.waves == 8) hipLaunchKernelGGL((tree_kernel<FMT, D, MB, 8>), grid, block, 0, stream, a, t);
+  else hipLaunchKernelGGL((tree_kernel<FMT, D, MB, 4>), grid, block, 0, stream, a, t);
 }
 
-template <int FMT>
+template <int FMT, int MB>
 static int launch_tree_f(const wmx_tree_args& a, unsigned blocks, const TreeLaunch& t, hipStream_t stream) {
   switch (a.head_dim) {
-    case 64: launch_tree_d<FMT, 64>(a, blocks, t, stream); return WMX_OK;
-    case 96: launch_tree_d<FMT, 96>(a, blocks, t, stream); return WMX_OK;
-    case 128: launch_tree_d<FMT, 128>(a, blocks, t, stream); return WMX_OK;
+    case 64: launch_tree_d<FMT, 64, MB>(a, blocks, t, stream); return WMX_OK;
+    case 96: launch_tree_d<FMT, 96, MB>(a, blocks, t, stream); return WMX_OK;
+    case 128: launch_tree_d<FMT, 128, MB>(a, blocks, t, stream); return WMX_OK;
     default: return WMX_E_UNSUPPORTED;
   }
 }
@@ -920,12 +926,13 @@ int launch_tree(const wmx_tree_args& a, hipStream_t stream) {
   const int64_t blocks = ((int64_t)t.ranges + 7) / 8 * 8 * t.tiles;
   const int64_t merged = (int64_t)a.batch * a.q_heads * a.nodes * (a.head_dim / 4);
   if (blocks > INT32_MAX || (merged + 255) / 256 > INT32_MAX || (int64_t)a.batch * a.kv_heads * max(1, t.nsplit) > INT32_MAX ||
-      (int64_t)t.share * max(1, t.nsplit) * kTreeStep > INT32_MAX)
+      (int64_t)t.share * max(1, t.nsplit) * t.waves * kTreeTile > INT32_MAX)
     return WMX_E_UNSUPPORTED;  // (ranges are counted, and begin, within 31 bits)
+  const bool narrow = tree_rows(a) == 16;
   int rc;
-  if (a.format == WMX_POOL_BF16) rc = launch_tree_f<WMX_POOL_BF16>(a, (unsigned)blocks, t, stream);
-  else if (a.format == WMX_POOL_E4M3) rc = launch_tree_f<WMX_POOL_E4M3>(a, (unsigned)blocks, t, stream);
-  else rc = launch_tree_f<WMX_POOL_INT8>(a, (unsigned)blocks, t, stream);
+  if (a.format == WMX_POOL_BF16) rc = narrow ? launch_tree_f<WMX_POOL_BF16, 1>(a, (unsigned)blocks, t, stream) : launch_tree_f<WMX_POOL_BF16, 2>(a, (unsigned)blocks, t, stream);
+  else if (a.format == WMX_POOL_E4M3) rc = narrow ? launch_tree_f<WMX_POOL_E4M3, 1>(a, (unsigned)blocks, t, stream) : launch_tree_f<WMX_POOL_E4M3, 2>(a, (unsigned)blocks, t, stream);
+  else rc = narrow ? launch_tree_f<WMX_POOL_INT8, 1>(a, (unsigned)blocks, t, stream) : launch_tree_f<WMX_POOL_INT8, 2>(a, (unsigned)blocks, t, stream);
   if (rc != WMX_OK || t.nsplit == 1) return rc;
   hipLaunchKernelGGL(tree_merge_kernel, dim3((unsigned)((merged + 255) / 256)), dim3(256), 0, stream, a, t, tree_rows(a), merged);
   return WMX_OK;
