@@ -803,12 +803,12 @@ typedef struct wmx_kv_read_args {
  * node i sees slot j < base_b, and slot base_b + a where tree_mask[b, i, a]
  * (no node without tree_mask), and of these the ones with key_mask[b, j] when
  * key_mask is given. Slots at or past `capacity` are never read. Rows with no
- * visible slot produce zeros.
+ * visible slot produce zeros. Over codes a weight times its slot's V scale has 11
+ * bits, or 2^-31 of the largest V scale of the slots read where it is smaller.
  * q (B, Hq, n, D) and o in bf16, strides [batch, head, node]; k/v pool strides
  * [batch, head, slot] in elements of the format, scales [batch, head] with unit
- * stride along the slots (WMX_POOL_BF16: none). Rows of q, o and of a bf16
- * pool are 16-byte aligned, rows of codes 8-byte aligned (16 for head_dim 64
- * and 128); a slot stride is below 2^25 bytes. With num_splits 0 the work is
+ * stride along the slots (WMX_POOL_BF16: none). Rows of q, o and the pools
+ * are 16-byte aligned; a slot stride is below 2^25 bytes. With num_splits 0 the work is
  * dealt out by the lengths (up to 256 batch rows).
  */
 typedef struct wmx_tree_args {

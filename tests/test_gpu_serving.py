@@ -9,6 +9,8 @@ fp32's, a bf16 rounding is off by at most 2^-8 of its value):
                    of unit normals are off by at most 2 D u sum_d |q_d k_d| <
                    1e-4, which moves a weight by as much: 2e-4 A. Products of
                    bf16 values with exactly converted codes add fp32 sums only.
+                   Over codes, weights times scales below fp16's normal range are off
+                   by 2^-25 where the largest scale is at least 32: 2^-30 of it.
   codes            half a step of the code at the exact quotient (e4m3: 2^-4 of
                    it, at least 2^-10; int8: 1/2) and what the fp32 value is off:
                    2^-22 of the quotient for values; for keys, whose norm sums D
@@ -404,6 +406,79 @@ def test_tree_attention_deals_ragged_batches(kind, capacity, batch, heads, kv_he
         torch.cuda.synchronize()
         _assert_tree(out, _tree_reference(query, k, v, at, tree, False, None, 0.2))
         assert torch.equal(out, eager)
+
+
+@pytest.mark.parametrize("kind", ["e4m3", "int8"])
+@pytest.mark.parametrize("nodes", [1, 20])
+@pytest.mark.parametrize("capacity", [700, 2800])
+@torch.no_grad()
+def test_tree_attention_scales_of_any_size(kind, nodes, capacity):
+    """V scales 2^16 apart, growing, falling and at random along the slots, around
+    2^-60, 1 and 2^60; K scales of no size at all and of 2^-60."""
+    gen = _gen(nodes + capacity)
+    key, value, _, _ = _pool_pair(gen, (2, 1, capacity, 64), kind)
+    query = _randn(gen, 2, 2, nodes, 64)
+    lengths = torch.tensor([capacity - nodes, 333])
+    tree = _random_tree(gen, nodes)
+    key.scales[:, :, 100:140] = 0.0
+    key.scales[:, :, 140:150] = 2.0**-60
+    ramp = torch.arange(capacity) * 17 // capacity - 8
+    for order in (ramp, ramp.flip(0), ramp[torch.randperm(capacity, generator=gen)]):
+        for size in (-60, 0, 60):
+            value.scales.copy_((2.0 ** (order + size)).float().expand(2, 1, -1))
+            out = tree_attention(query, key, value, kv_lengths=lengths.to(DEV), tree_mask=tree)
+            exact, total = _tree_reference(query, _values(key), _values(value), lengths, tree, False, None, 0.125)
+            assert torch.isfinite(out.float()).all()
+            small = capacity * 2.0**-30 * 448 * 2.0 ** (8 + size)
+            far = (out.to(F64) - exact).abs() - 2**-8 * exact.abs() - (2**-8 + 2e-4) * total - small
+            assert (far <= 0).all(), (kind, size, far.max().item())
+
+
+@torch.no_grad()
+def test_tree_attention_of_nothing():
+    """No slots, no nodes, no rows, more key ranges than the pool has steps."""
+    gen = _gen(8)
+    for kind in ("bf16", "e4m3", "int8"):
+        key, value, k, v = _pool_pair(gen, (2, 2, 40, 64), kind)
+        cut = [kv_pool.QuantizedPool(p.codes[:, :, :0], p.scales[:, :, :0]) if kind != "bf16" else p[:, :, :0] for p in (key, value)]
+        query = _randn(gen, 2, 4, 3, 64)
+        own = tree_mask_from_parents([-1, 0, 0], device=DEV)[0]
+        assert (tree_attention(query, *cut, kv_lengths=5, tree_mask=own) == 0).all()
+        assert tree_attention(query[:, :, :0], key, value, kv_lengths=5).shape == (2, 0, 4, 64)
+        assert tree_attention(query[:0], *(p.select(1, 0)[:0, None] if kind == "bf16" else kv_pool.QuantizedPool(*(t[:0] for t in p)) for p in (key, value)),
+                              kv_lengths=5).shape == (0, 3, 4, 64)
+        many = tree_attention(query, key, value, kv_lengths=17, tree_mask=own, num_splits=2**31 - 1)
+        _assert_tree(many, _tree_reference(query, k, v, [17, 17], own, False, None, 0.125))
+    pool = kv_pool.quantize_pool(_randn(gen, 1, 1, 1, 0, 96))
+    assert kv_pool.read_pool(pool).shape == (1, 1, 1, 0, 96)
+    scores = token_log_probs(_randn(gen, 0, 50), torch.zeros(0, dtype=torch.long, device=DEV), top_k=3)
+    assert scores.log_probs.shape == (0,) and scores.top_indices.shape == (0, 3)
+
+
+def test_forward_only_calls_refuse_gradients():
+    """Queries, rows and scales that need a gradient, on the GPU."""
+    pool = kv_pool.quantize_pool(_randn(_gen(1), 1, 1, 2, 30, 64))
+    channel, rows = pool.select(1, 0), _randn(_gen(2), 1, 1, 2, 4, 64)
+    query = _randn(_gen(3), 1, 2, 1, 64)
+    grown = kv_pool.QuantizedPool(channel.codes, channel.scales.clone().requires_grad_())
+    for args in ((query.clone().requires_grad_(), channel, channel), (query, grown, channel), (query, channel, grown)):
+        with pytest.raises(RuntimeError, match="forward-only"):
+            tree_attention(*args, kv_lengths=20)
+    with pytest.raises(RuntimeError, match="forward-only"):
+        kv_pool.quantize_pool(rows.clone().requires_grad_())
+    with pytest.raises(RuntimeError, match="forward-only"):
+        kv_pool.read_pool(kv_pool.QuantizedPool(pool.codes, pool.scales.clone().requires_grad_()))
+
+
+def test_tree_attention_refuses_unaligned_rows():
+    """Rows of codes that do not start 16-byte aligned, before any launch."""
+    whole = kv_pool.quantize_pool(_randn(_gen(1), 1, 1, 1, 40, 96)).select(1, 0)
+    shifted = torch.zeros(1, 1, 30, 104, dtype=torch.uint8, device=DEV).view(E4M3)[..., 8:]
+    bad = kv_pool.QuantizedPool(shifted, whole.scales[:, :, :30])
+    query = _randn(_gen(2), 1, 1, 1, 96)
+    for pair in ((bad, bad), (kv_pool.QuantizedPool(whole.codes[:, :, :30], bad.scales), bad)):
+        with pytest.raises(RuntimeError, match="16-byte aligned"):
+            tree_attention(query, *pair, kv_lengths=20)
 
 
 @pytest.mark.parametrize("kind", ["bf16", "int8"])

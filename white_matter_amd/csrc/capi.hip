@@ -740,10 +740,8 @@ int wmx_tree_attn(const wmx_tree_args* a, void* stream) {
     return fail(WMX_E_INVALID, "tree attention pointer is NULL");
   if (!aligned16(a->q) || !strides_vec8(a->q_stride, 3)) return fail(WMX_E_INVALID, "q must be 16-byte aligned rows");
   if (!aligned16(a->o) || !strides_vec8(a->o_stride, 3)) return fail(WMX_E_INVALID, "o must be 16-byte aligned rows");
-  // rows of codes are read 16 bytes at a time, at head_dim 96 8 bytes
-  const int64_t unit = !codes ? 8 : a->head_dim == 96 ? 8 : 16;
-  const uintptr_t low = (codes && a->head_dim == 96) ? 7u : 15u;
-  if (((uintptr_t)a->k & low) || ((uintptr_t)a->v & low)) return fail(WMX_E_INVALID, "pool rows must be 16-byte aligned");
+  const int64_t unit = codes ? 16 : 8;  // rows are read 16 bytes at a time
+  if (!aligned16(a->k) || !aligned16(a->v)) return fail(WMX_E_INVALID, "pool rows must be 16-byte aligned");
   for (const int64_t* st : {a->k_stride, a->v_stride}) {
     for (int i = 0; i < 3; ++i)
       if (st[i] % unit) return fail(WMX_E_INVALID, "pool rows must be 16-byte aligned");

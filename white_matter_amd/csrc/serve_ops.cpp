@@ -190,6 +190,7 @@ void kv_quant_store(const optional<Tensor>& key, const optional<Tensor>& value, 
 
 Tensor kv_quant_read(const Tensor& codes, const Tensor& scales, const optional<Tensor>& slots) {
   check_pool(codes, scales, codes.device(), 5);
+  forward_only("the pool read", {&scales});
   wmx_kv_read_args a;
   std::memset(&a, 0, sizeof(a));
   TORCH_CHECK_VALUE(!slots || slots->dim() >= 1, "slots must be (T,) or (B, T)");
@@ -237,7 +238,7 @@ void tree_attention_check(const Tensor& query, const Tensor& key, const Tensor& 
                     "Q/K/V require matching batch/head_dim and divisible heads");
   TORCH_CHECK_VALUE(key.device() == query.device() && value.device() == query.device(), "Q/K/V must share a device");
   TORCH_CHECK_VALUE(at::isFloatingType(query.scalar_type()), "queries must be floating point");
-  forward_only("tree_attention", {&query, &key, &value});
+  forward_only("tree_attention", {&query, &key, &value, given(key_scales), given(value_scales)});
   TORCH_CHECK_VALUE(!kv_lengths || (kv_lengths->dim() == 1 && kv_lengths->size(0) == batch &&
                                     (kv_lengths->scalar_type() == at::kLong || kv_lengths->scalar_type() == at::kInt)),
                     "kv_lengths must be an integer or integer (B,)");

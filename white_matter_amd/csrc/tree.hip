@@ -33,7 +33,9 @@ namespace wmx {
 // rescale nothing.
 constexpr float kLazyMax = 8.f;
 // V scales times 2^lv stay at most 64, so that weights times scales stay below
-// 2^14 in fp16 (largest 65,504).
+// 2^14 in fp16 (largest 65,504). Its smallest step is 2^-24: a weight of one takes
+// its full bits on scales down to 2^-20 of the largest, and an error of 2^-31 of the
+// largest is the most there is below.
 constexpr float kScaleRoom = 64.f;
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
@@ -889,6 +891,7 @@ static TreeLaunch tree_plan(const wmx_tree_args& a) {
   t.waves = t.nsplit == 1 && pairs * tiles <= kCUs ? 8 : 4;
   const int64_t step = t.waves * kTreeTile, most = max((int64_t)1, (a.capacity + step - 1) / step);  // steps of a (row, head)
   if (t.nsplit > 0) {
+    t.nsplit = (int)min((int64_t)t.nsplit, most);  // (more would be empty)
     t.share = (int)((most + t.nsplit - 1) / t.nsplit);
     t.ranges = (int)min((int64_t)INT32_MAX, pairs * t.nsplit);
   } else {

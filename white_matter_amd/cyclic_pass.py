@@ -669,6 +669,8 @@ def score_drafts(
     parents = torch.as_tensor(parents)
     tree_mask, depths = tree_mask_from_parents(parents, device="cpu")
     passes = int(depths.max()) + 1 if passes is None else passes
+    if passes < 1:
+        raise ValueError("passes must be positive")
     tree_mask, depths = tree_mask.to(device), depths.to(device)
     x = model.embed[tokens].to(model.residual_dtype)
     rope = model.rope((position.reshape(-1, 1) + depths).expand(batch, nodes) + offset)
