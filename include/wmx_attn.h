@@ -733,8 +733,8 @@ enum {
  * values, both computed in fp32 without intermediate rounding, quantised into
  * pool slots. Either side may be absent (key and key_codes NULL, or value and
  * value_codes). Token t of batch row b goes to slot slots[b * slots_stride + t]
- * (slots NULL: slot t); a slot outside [0, pool_slots) is skipped. Without
- * weight, cos and sin (all NULL) the keys are quantised as they are.
+ * (slots NULL: slot t); a slot outside [0, pool_slots) is skipped. Keys come with
+ * weight, cos and sin.
  * Element strides [batch, channel, head, token or slot]; code strides in bytes,
  * multiples of 8, unit stride along D; sources 16-byte aligned rows as
  * wmx_kv_store_args. head_dim 64, 96 or 128.

@@ -687,8 +687,8 @@ int wmx_kv_quant_store(const wmx_kv_quant_args* a, void* stream) {
   if (!a->key && !a->value) return fail(WMX_E_INVALID, "quantised store has neither keys nor values");
   if (!a->key != !a->key_codes || !a->key != !a->key_scales || !a->value != !a->value_codes || !a->value != !a->value_scales)
     return fail(WMX_E_INVALID, "a side's rows, codes and scales are given together");
-  if (!a->k_norm_weight != !a->cos || !a->cos != !a->sin || (a->cos && !a->key))
-    return fail(WMX_E_INVALID, "the norm weight, cos and sin are given together, with keys");
+  if (!a->key != !a->k_norm_weight || !a->key != !a->cos || !a->key != !a->sin)
+    return fail(WMX_E_INVALID, "keys come with a norm weight, cos and sin");
   if (!a->slots && a->tokens > a->pool_slots) return fail(WMX_E_INVALID, "more tokens than slots, and no slots given");
   if (!aligned16(a->key) || !aligned16(a->value) || !aligned16(a->k_norm_weight) || !aligned16(a->cos) || !aligned16(a->sin) ||
       !aligned8(a->slots) || !aligned8(a->key_codes) || !aligned8(a->value_codes))

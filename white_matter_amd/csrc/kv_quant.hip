@@ -67,7 +67,7 @@ __device__ __forceinline__ u32x2 quantise_row(float (&x)[8], float& scale) {
 // group's heads, one at a time: 71 registers leave seven waves a SIMD, whose loads
 // overlap (the 829 MB above with four heads' loads in flight 197 us, and few heads
 // per thread 20 us where one at a time takes 9.6).
-template <int D, int FMT, bool KEY, bool ROPE, bool VALUE>
+template <int D, int FMT, bool KEY, bool VALUE>
 __global__ __launch_bounds__(256) void kv_quant_kernel(const wmx_kv_quant_args a, int64_t tokens_total, int head_groups) {
   constexpr int LD = D / 8;           // lanes holding data
   constexpr int L = LD <= 8 ? 8 : 16; // lanes per row (a power of two; D = 96 leaves 4 idle)
@@ -92,7 +92,7 @@ __global__ __launch_bounds__(256) void kv_quant_kernel(const wmx_kv_quant_args a
   const int dl = data ? d0 : 0;
 
   float w[8], cs[8], sn[8];
-  if constexpr (KEY && ROPE) {
+  if constexpr (KEY) {
     load8(a.k_norm_weight, (int64_t)c * D + dl, a.weight_dtype == WMX_DTYPE_BF16, w);
     const int64_t ro = a.rope_by_slot ? (slot_ok ? slot : 0) * a.rope_stride[1] + dl
                                       : (int64_t)b * a.rope_stride[0] + (int64_t)t * a.rope_stride[1] + dl;
@@ -124,22 +124,20 @@ __global__ __launch_bounds__(256) void kv_quant_kernel(const wmx_kv_quant_args a
       }
     };
     if constexpr (KEY) {
-      if constexpr (ROPE) {
-        float ss = 0.f;
+      float ss = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-        if (!data) ss = 0.f;
+      for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+      if (!data) ss = 0.f;
 #pragma unroll
-        for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
-        const float inv = 1.f / sqrtf(ss / (float)D + a.eps);
-        float y[8];
+      for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor(ss, o);
+      const float inv = 1.f / sqrtf(ss / (float)D + a.eps);
+      float y[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = x[e] * inv * w[e];
+      for (int e = 0; e < 8; ++e) y[e] = x[e] * inv * w[e];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const float other = __shfl(y[e], data ? partner : 0);
-          x[e] = fmaf(low ? -other : other, sn[e], y[e] * cs[e]);
-        }
+      for (int e = 0; e < 8; ++e) {
+        const float other = __shfl(y[e], data ? partner : 0);
+        x[e] = fmaf(low ? -other : other, sn[e], y[e] * cs[e]);
       }
       put(x, a.key_codes, a.key_codes_stride, a.key_scales, a.key_scales_stride);
     }
@@ -149,17 +147,12 @@ __global__ __launch_bounds__(256) void kv_quant_kernel(const wmx_kv_quant_args a
 
 template <int D, int FMT>
 static void launch_kv_quant_d(const wmx_kv_quant_args& a, int64_t rows, int groups, dim3 grid, hipStream_t stream) {
-  const bool rope = a.k_norm_weight != nullptr;
   if (!a.key)
-    hipLaunchKernelGGL((kv_quant_kernel<D, FMT, false, false, true>), grid, dim3(256), 0, stream, a, rows, groups);
-  else if (rope && a.value)
-    hipLaunchKernelGGL((kv_quant_kernel<D, FMT, true, true, true>), grid, dim3(256), 0, stream, a, rows, groups);
-  else if (rope)
-    hipLaunchKernelGGL((kv_quant_kernel<D, FMT, true, true, false>), grid, dim3(256), 0, stream, a, rows, groups);
+    hipLaunchKernelGGL((kv_quant_kernel<D, FMT, false, true>), grid, dim3(256), 0, stream, a, rows, groups);
   else if (a.value)
-    hipLaunchKernelGGL((kv_quant_kernel<D, FMT, true, false, true>), grid, dim3(256), 0, stream, a, rows, groups);
+    hipLaunchKernelGGL((kv_quant_kernel<D, FMT, true, true>), grid, dim3(256), 0, stream, a, rows, groups);
   else
-    hipLaunchKernelGGL((kv_quant_kernel<D, FMT, true, false, false>), grid, dim3(256), 0, stream, a, rows, groups);
+    hipLaunchKernelGGL((kv_quant_kernel<D, FMT, true, false>), grid, dim3(256), 0, stream, a, rows, groups);
 }
 
 int launch_kv_quant(const wmx_kv_quant_args& a, hipStream_t stream) {

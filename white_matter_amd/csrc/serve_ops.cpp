@@ -138,8 +138,9 @@ void kv_quant_store(const optional<Tensor>& key, const optional<Tensor>& value, 
     a.pool_slots = (int32_t)n[3];
     a.format = pool_format(*s.codes);
   }
+  TORCH_CHECK_VALUE(key.has_value() == weight.has_value() && key.has_value() == cos.has_value() && key.has_value() == sin.has_value(),
+                    "keys come with a norm weight, cos and sin");
   if (weight) {
-    TORCH_CHECK_VALUE(key && cos && sin, "a key norm comes with keys, cos and sin");
     TORCH_CHECK_VALUE(weight->dim() == 2 && weight->size(0) == channels && weight->size(1) == dim && weight->device() == first.device(),
                       "k_norm_weight must be (C, D)");
     const bool tables = rope_by_slot ? cos->dim() == 2 && cos->size(0) == a.pool_slots && cos->size(1) == dim
@@ -149,8 +150,6 @@ void kv_quant_store(const optional<Tensor>& key, const optional<Tensor>& value, 
                       "cos and sin must be (B, T, D), or with rope_by_slot (N, D) tables, of one dtype");
     source_dtype(*weight);
     source_dtype(*cos);
-  } else {
-    TORCH_CHECK_VALUE(!cos && !sin && (!key || !value || slots), "keys without a norm weight take no cos and sin");
   }
   const Tensor at_slots = slot_rows(slots, batch, tokens, first, a.slots_stride);
   TORCH_CHECK(first.is_cuda(), "the quantised pool write runs on the HIP kernels: it takes GPU tensors");

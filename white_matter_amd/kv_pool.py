@@ -238,9 +238,8 @@ def read_pool(pool: QuantizedPool, slots: torch.Tensor | None = None) -> torch.T
 
 
 # kv_quant_store(key, value, weight, cos, sin, slots, key_codes, key_scales,
-#     value_codes, value_scales, rope_by_slot, eps) -> (): either side None;
-#     without weight, cos and sin the rows are quantised as they are; without
-#     slots token t goes to slot t
+#     value_codes, value_scales, rope_by_slot, eps) -> (): either side None,
+#     weight, cos and sin with keys; without slots token t goes to slot t
 _store = torch.ops.white_matter.kv_quant_store.default
 # kv_quant_read(codes, scales, slots) -> (B, C, H, T, D) bf16
 _read = torch.ops.white_matter.kv_quant_read.default
