@@ -435,6 +435,36 @@ def test_tree_attention_scales_of_any_size(kind, nodes, capacity):
 
 
 @torch.no_grad()
+def test_calls_on_two_streams_at_once():
+    """Dealt and split attention and scores on two streams, each with workspaces of
+    its own, against the same calls alone."""
+    gen = _gen(21)
+    key, value, _, _ = _pool_pair(gen, (3, 2, 5200, 64), "e4m3")
+    lengths = torch.tensor([5100, 40, 2600], device=DEV)
+    queries = [_randn(gen, 3, 4, 5, 64) for _ in range(2)]
+    tree = _random_tree(gen, 5)
+    logits = [_randn(gen, 7, 33001) for _ in range(2)]
+    tokens = torch.randint(0, 33001, (7,), generator=gen).to(DEV)
+
+    def calls(i):
+        outs = [tree_attention(queries[i], key, value, kv_lengths=lengths, tree_mask=tree, num_splits=n) for n in (0, 3)]
+        return [*outs, *token_log_probs(logits[i], tokens, top_k=5)]
+
+    alone = [calls(i) for i in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    together = [[], []]
+    for _ in range(4):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                together[i].append(calls(i))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for got in together[i]:
+            assert all(torch.equal(a, b) for a, b in zip(got, alone[i]))
+
+
+@torch.no_grad()
 def test_tree_attention_of_nothing():
     """No slots, no nodes, no rows, more key ranges than the pool has steps."""
     gen = _gen(8)

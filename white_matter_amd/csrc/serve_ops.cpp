@@ -227,7 +227,8 @@ void tree_attention_check(const Tensor& query, const Tensor& key, const Tensor& 
     check_pool(value, *value_scales, query.device(), 4);
     TORCH_CHECK_VALUE(key.scalar_type() == value.scalar_type(), "key and value codes must be of one type");
   } else {
-    TORCH_CHECK_VALUE(at::isFloatingType(key.scalar_type()) && at::isFloatingType(value.scalar_type()) && key.element_size() > 1 && value.element_size() > 1,
+    TORCH_CHECK_VALUE(at::isFloatingType(key.scalar_type()) && at::isFloatingType(value.scalar_type()) && key.element_size() > 1 &&
+                          value.element_size() > 1,
                       "keys and values must be floating point, or quantised pools");
   }
   TORCH_CHECK_VALUE(query.dim() == 4 && key.dim() == 4 && key.sizes() == value.sizes(), "Q/K/V require (B,H,T,D) tensors with matching K/V");

@@ -875,10 +875,9 @@ __global__ __launch_bounds__(256) void tree_merge_kernel(const wmx_tree_args a, 
   *(u32x2*)out = w;
 }
 
-// Query rows per workgroup: 16 or 32. Two 16s use 240 registers, two waves a
-// SIMD; three and four share the conversions further but leave one wave a SIMD
-// (measured: 64 nodes x 2 heads over 16 x 8,192 slots 128 us with two, 167 with
-// four, 194 with three).
+// Query rows per workgroup: 16 or 32. Two 16s use up to 232 registers, two waves a
+// SIMD; three and four share the conversions further but leave one wave a SIMD, and
+// took 1.5 and 1.3 times as long (64 nodes x 2 heads over 16 x 8,192 slots).
 static int tree_rows(const wmx_tree_args& a) { return (int64_t)a.nodes * (a.q_heads / a.kv_heads) <= 16 ? 16 : 32; }
 
 static TreeLaunch tree_plan(const wmx_tree_args& a) {
@@ -908,18 +907,24 @@ int64_t tree_workspace_size(const wmx_tree_args& a) {
 }
 
 template <int FMT, int D, int MB>
-static void launch_tree_d(const wmx_tree_args& a, unsigned blocks, const TreeLaunch& t, hipStream_t stream) {
+static void launch_tree_m(const wmx_tree_args& a, unsigned blocks, const TreeLaunch& t, hipStream_t stream) {
   const dim3 grid(blocks), block(64 * t.waves);
   if (t.waves == 8) hipLaunchKernelGGL((tree_kernel<FMT, D, MB, 8>), grid, block, 0, stream, a, t);
   else hipLaunchKernelGGL((tree_kernel<FMT, D, MB, 4>), grid, block, 0, stream, a, t);
 }
 
-template <int FMT, int MB>
+template <int FMT, int D>
+static void launch_tree_d(const wmx_tree_args& a, unsigned blocks, const TreeLaunch& t, hipStream_t stream) {
+  if (tree_rows(a) == 16) launch_tree_m<FMT, D, 1>(a, blocks, t, stream);
+  else launch_tree_m<FMT, D, 2>(a, blocks, t, stream);
+}
+
+template <int FMT>
 static int launch_tree_f(const wmx_tree_args& a, unsigned blocks, const TreeLaunch& t, hipStream_t stream) {
   switch (a.head_dim) {
-    case 64: launch_tree_d<FMT, 64, MB>(a, blocks, t, stream); return WMX_OK;
-    case 96: launch_tree_d<FMT, 96, MB>(a, blocks, t, stream); return WMX_OK;
-    case 128: launch_tree_d<FMT, 128, MB>(a, blocks, t, stream); return WMX_OK;
+    case 64: launch_tree_d<FMT, 64>(a, blocks, t, stream); return WMX_OK;
+    case 96: launch_tree_d<FMT, 96>(a, blocks, t, stream); return WMX_OK;
+    case 128: launch_tree_d<FMT, 128>(a, blocks, t, stream); return WMX_OK;
     default: return WMX_E_UNSUPPORTED;
   }
 }
@@ -931,11 +936,10 @@ int launch_tree(const wmx_tree_args& a, hipStream_t stream) {
   if (blocks > INT32_MAX || (merged + 255) / 256 > INT32_MAX || (int64_t)a.batch * a.kv_heads * max(1, t.nsplit) > INT32_MAX ||
       (int64_t)t.share * max(1, t.nsplit) * t.waves * kTreeTile > INT32_MAX)
     return WMX_E_UNSUPPORTED;  // (ranges are counted, and begin, within 31 bits)
-  const bool narrow = tree_rows(a) == 16;
   int rc;
-  if (a.format == WMX_POOL_BF16) rc = narrow ? launch_tree_f<WMX_POOL_BF16, 1>(a, (unsigned)blocks, t, stream) : launch_tree_f<WMX_POOL_BF16, 2>(a, (unsigned)blocks, t, stream);
-  else if (a.format == WMX_POOL_E4M3) rc = narrow ? launch_tree_f<WMX_POOL_E4M3, 1>(a, (unsigned)blocks, t, stream) : launch_tree_f<WMX_POOL_E4M3, 2>(a, (unsigned)blocks, t, stream);
-  else rc = narrow ? launch_tree_f<WMX_POOL_INT8, 1>(a, (unsigned)blocks, t, stream) : launch_tree_f<WMX_POOL_INT8, 2>(a, (unsigned)blocks, t, stream);
+  if (a.format == WMX_POOL_BF16) rc = launch_tree_f<WMX_POOL_BF16>(a, (unsigned)blocks, t, stream);
+  else if (a.format == WMX_POOL_E4M3) rc = launch_tree_f<WMX_POOL_E4M3>(a, (unsigned)blocks, t, stream);
+  else rc = launch_tree_f<WMX_POOL_INT8>(a, (unsigned)blocks, t, stream);
   if (rc != WMX_OK || t.nsplit == 1) return rc;
   hipLaunchKernelGGL(tree_merge_kernel, dim3((unsigned)((merged + 255) / 256)), dim3(256), 0, stream, a, t, tree_rows(a), merged);
   return WMX_OK;
